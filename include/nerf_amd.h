@@ -128,6 +128,59 @@ int nerf_weight_gradient_bf16(const unsigned short* d_err, int rows_out, int ld_
                               int cols, int ld_act, long batch, float* d_dW, float* d_workspace,
                               size_t workspace_bytes, int accumulate);
 
+/* ---- optimizer over many tensors.  No counterpart in the reference, whose update_weights_mlp works on the two
+ * matrices of one MLP (train.c:219-220): a list of tensors of any number, sizes and alignment is updated by ONE
+ * launch, with the states in 32 or in 8 bits, after an optional clip by the global norm of the gradients. -------- */
+enum { NERF_TYPE_F32 = 0, NERF_TYPE_BF16 = 1 };
+#define NERF_ADAMW_MAX_ELEMENTS ((size_t)1 << 40) /* of one tensor */
+typedef struct {
+    float* w;              /* weights [n] */
+    const void* g;         /* gradients [n], of grad_type */
+    void* m;               /* first moments:  float [n], or 8-bit codes [n] */
+    void* v;               /* second moments: float [n], or 8-bit codes [n] of their square roots */
+    unsigned char* m_exp;  /* 8-bit states only: one exponent per 256 elements, [nerf_adamw_state_blocks(n)] */
+    unsigned char* v_exp;
+    unsigned short* w_bf16; /* NULL, or [n]: also receives the new weights rounded to bf16 */
+    size_t n;              /* 0: the tensor is passed over, its pointers are not read */
+    int grad_type;         /* NERF_TYPE_F32 or NERF_TYPE_BF16 */
+    float lr_scale;        /* the step's learning rate is multiplied by it (1 for most) */
+    float weight_decay;    /* NERF_ADAM_WEIGHT_DECAY is the MLP's; 0 for none */
+} NerfAdamwTensor;
+typedef struct NerfAdamw NerfAdamw;
+/* blocks of 256 elements in a tensor of n */
+size_t nerf_adamw_state_blocks(size_t n);
+/* A plan over `count` tensors on the current device.  state_bits: 32, 8, or 0 for a plan that only takes norms (it
+ * reads g, grad_type and n of each tensor).  The list is copied; its pointers (device memory, aligned to their
+ * elements) must stay valid while the plan is used, and their contents are the caller's.  Zeroed states are the
+ * start.  Returns 1 for a bad argument: among them a buffer that a step writes and that overlaps another one of
+ * the list, and a pointer to pageable host memory or another GPU. */
+int nerf_adamw_create(const NerfAdamwTensor* tensors, int count, int state_bits, float beta1, float beta2, float eps,
+                      NerfAdamw** out);
+/* waits for the device's work and frees the plan's own tables */
+void nerf_adamw_destroy(NerfAdamw* plan);
+/* Step number `step` (1, 2, ...) on every tensor of the plan:
+ *   g' = g / grad_div, times max_norm / *d_norm where d_norm is given and *d_norm > max_norm
+ *   m = beta1 m + (1 - beta1) g';  v = beta2 v + (1 - beta2) g'^2;  lr = learning_rate * lr_scale
+ *   w = w (1 - lr weight_decay) - lr sqrt(1 - beta2^step) / (1 - beta1^step) m / (sqrt(v) + eps)
+ * in 32 bits, in the order of nerf_trainer_update: without d_norm, and with 32-bit states, the same bits.  Where
+ * *d_norm is not finite nothing is changed, on any tensor.
+ * 8-bit states: w is updated from the new moments in 32 bits; m and sqrt(v) are then rounded to 8 bits, m to a sign,
+ * 4 exponent bits and 3 mantissa bits, sqrt(v) to 4 and 4, below a power of two per 256 elements (its biased exponent
+ * in m_exp / v_exp).  seed 0 rounds to nearest (ties away from zero); another seed rounds up or down by chance, a
+ * pure function of (seed, step, place in the list, element), so that changes smaller than a rounding step are not
+ * lost on average: what training wants, as v moves by a thousandth a step.  A sqrt(v) that is not zero stays so; a
+ * moment that is not finite is held as zero.  seed is not used with 32-bit states.
+ * d_norm: one float on the device (nerf_grad_norm) or NULL; then max_norm is not used.
+ * Returns 1 while the stream is being captured: a graph would repeat this step number and learning rate. */
+int nerf_adamw_step(NerfAdamw* plan, int step, float learning_rate, float grad_div, const float* d_norm, float max_norm,
+                    unsigned long long seed);
+/* The values that the 8-bit states stand for, of all tensors back to back in the list's order, as bf16 (each is one
+ * exactly): d_m and d_root_v [sum of n], either may be NULL. */
+int nerf_adamw_read_states(NerfAdamw* plan, unsigned short* d_m, unsigned short* d_root_v);
+/* *d_norm = sqrt(sum of all squared gradients of the plan) / grad_div; summed in 64 bits in a fixed order (the same
+ * bits on every call).  Uses buffers of the plan: calls on one plan must not overlap on two streams. */
+int nerf_grad_norm(NerfAdamw* plan, float grad_div, float* d_norm);
+
 /* ---- dataset on the device -------------------------------------------------------------------- */
 typedef struct NerfDeviceDataset NerfDeviceDataset;
 /* copies every camera and every image's RGBA8 pixels of a Dataset (data.h:25-29) to the device */

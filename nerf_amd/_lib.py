@@ -72,6 +72,14 @@ class NerfTrainerConfig(C.Structure):  # include/nerf_amd.h
     ]
 
 
+class NerfAdamwTensor(C.Structure):  # include/nerf_amd.h
+    _fields_ = [
+        ("w", C.c_void_p), ("g", C.c_void_p), ("m", C.c_void_p), ("v", C.c_void_p),
+        ("m_exp", C.c_void_p), ("v_exp", C.c_void_p), ("w_bf16", C.c_void_p),
+        ("n", C.c_size_t), ("grad_type", C.c_int), ("lr_scale", C.c_float), ("weight_decay", C.c_float),
+    ]
+
+
 VP = C.c_void_p
 _SIGS = {
     # runtime
@@ -119,6 +127,14 @@ _SIGS = {
     "nerf_weight_gradient_bf16_workspace": (C.c_size_t, [C.c_int, C.c_int, C.c_long]),
     "nerf_weight_gradient_bf16": (C.c_int, [VP, C.c_int, C.c_int, VP, C.c_int, C.c_int, C.c_long, VP, VP, C.c_size_t,
                                             C.c_int]),
+    # optimizer over many tensors
+    "nerf_adamw_state_blocks": (C.c_size_t, [C.c_size_t]),
+    "nerf_adamw_create": (C.c_int, [C.POINTER(NerfAdamwTensor), C.c_int, C.c_int, C.c_float, C.c_float, C.c_float,
+                                    C.POINTER(VP)]),
+    "nerf_adamw_destroy": (None, [VP]),
+    "nerf_adamw_step": (C.c_int, [VP, C.c_int, C.c_float, C.c_float, VP, C.c_float, C.c_ulonglong]),
+    "nerf_adamw_read_states": (C.c_int, [VP, VP, VP]),
+    "nerf_grad_norm": (C.c_int, [VP, C.c_float, VP]),
     # dataset / encode
     "nerf_dataset_upload": (VP, [C.POINTER(Dataset)]),
     "nerf_dataset_upload_cameras": (VP, [C.POINTER(Dataset)]),

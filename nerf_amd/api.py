@@ -315,6 +315,59 @@ class Trainer:
         return rgb8, pix
 
 
+# ---- optimizer over many tensors -------------------------------------------------------------------
+
+def _ptr(x):
+    """a device address: of an object with .ptr (DeviceArray), or the number itself; None is NULL"""
+    return getattr(x, "ptr", x) or 0
+
+
+class AdamW:
+    """nerf_adamw_* and nerf_grad_norm of include/nerf_amd.h: AdamW over a list of tensors in one launch.
+
+    tensors: dicts with g and n, and (unless state_bits is 0: norms only) w, m, v, for 8-bit states also m_exp and
+    v_exp; optional w_bf16, g_bf16 (the gradients are bf16), lr_scale (1) and weight_decay (the MLP's 0.01).  Addresses
+    are DeviceArrays or integers; what they point to has to outlive this object (DeviceArrays are kept alive)."""
+
+    _ADDRESSES = ("w", "g", "m", "v", "m_exp", "v_exp", "w_bf16")
+
+    def __init__(self, tensors, state_bits=32, beta1=0.9, beta2=0.999, eps=1e-8):
+        self.handle = None
+        self._keep = list(tensors)
+        table = (_lib.NerfAdamwTensor * max(1, len(self._keep)))()
+        for t, s in zip(self._keep, table):
+            extra = set(t) - set(self._ADDRESSES) - {"n", "g_bf16", "lr_scale", "weight_decay"}
+            if extra:
+                raise TypeError(f"AdamW tensors have no {sorted(extra)}")
+            for name in self._ADDRESSES:
+                setattr(s, name, _ptr(t.get(name)))
+            s.n, s.grad_type = t["n"], int(bool(t.get("g_bf16")))
+            s.lr_scale, s.weight_decay = t.get("lr_scale", 1.0), t.get("weight_decay", 0.01)
+        out = C.c_void_p()
+        _check(lib.nerf_adamw_create(table, len(self._keep), state_bits, beta1, beta2, eps, C.byref(out)), "nerf_adamw_create")
+        self.handle = out.value
+
+    def destroy(self):
+        if self.handle:
+            lib.nerf_adamw_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.destroy()
+        except Exception:
+            pass
+
+    def step(self, step, lr, grad_div=1.0, norm=None, max_norm=0.0, seed=0):
+        _check(lib.nerf_adamw_step(self.handle, step, lr, grad_div, _ptr(norm), max_norm, seed), "nerf_adamw_step")
+
+    def grad_norm(self, norm, grad_div=1.0):
+        _check(lib.nerf_grad_norm(self.handle, grad_div, _ptr(norm)), "nerf_grad_norm")
+
+    def read_states(self, m=None, root_v=None):
+        _check(lib.nerf_adamw_read_states(self.handle, _ptr(m), _ptr(root_v)), "nerf_adamw_read_states")
+
+
 # ---- per-kernel timing -----------------------------------------------------------------------------
 
 def prof_read():

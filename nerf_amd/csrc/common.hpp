@@ -42,6 +42,9 @@ enum KernelId {
     K_COMPOSITE_BWD,
     K_ADAMW,
     K_GEMM_PAIR,  // a weight gradient and the data gradient that follows it as one launch (GemmPairScope)
+    K_GRAD_NORM,
+    K_QUANTIZE_W4,
+    K_GEMM_W4,
     K_COUNT
 };
 struct ProfScope {

@@ -24,7 +24,8 @@ double g_prof_work[K_COUNT];
 long g_prof_launches[K_COUNT];
 const char* const g_prof_names[K_COUNT] = {
     "encode",        "gemm_fwd",     "gemm_dgrad",     "gemm_wgrad", "reduce_slabs", "skinny_fwd",
-    "skinny_bwd",    "composite_fwd", "loss_reduce",   "composite_bwd", "adamw",      "gemm_pair"};
+    "skinny_bwd",    "composite_fwd", "loss_reduce",   "composite_bwd", "adamw",      "gemm_pair",
+    "grad_norm",     "quantize_w4",   "gemm_w4"};
 thread_local bool g_prof_discard = false;
 thread_local int g_prof_redirect = -1;
 thread_local double g_prof_extra = 0.0;
