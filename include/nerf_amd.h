@@ -181,6 +181,29 @@ int nerf_adamw_read_states(NerfAdamw* plan, unsigned short* d_m, unsigned short*
  * bits on every call).  Uses buffers of the plan: calls on one plan must not overlap on two streams. */
 int nerf_grad_norm(NerfAdamw* plan, float grad_div, float* d_norm);
 
+/* ---- weights in 4 bits, for a trained model that answers a few points at a time.  No counterpart in the reference.
+ * A [rows][cols] matrix is held as codes [rows][nerf_w4_row_bytes(cols)] -- two to a byte, the lower four bits first,
+ * sign and magnitude 0, 0.5, 1, 1.5, 2, 3, 4, 6 (codes 0..7; plus 8 for negative) -- and one bf16 scale per `group`
+ * (32, 64 or 128) consecutive columns of a row, [rows][ceil(cols / group)].  A weight is code value * scale. ---- */
+size_t nerf_w4_row_bytes(int cols); /* 16 bytes per 32 columns, rounded up */
+/* scale = the smallest bf16 with 6 scale >= largest |weight| of the group, codes to nearest with ties to the even
+ * code.  A group that holds a weight that is not finite gets a NaN scale.  Rows of d_src are ld_src >= cols floats
+ * apart; codes behind the last column are zero.  d_codes must be 16-byte aligned. */
+int nerf_quantize_w4(const float* d_src, long ld_src, int rows, int cols, int group, unsigned char* d_codes,
+                     unsigned short* d_scales);
+/* the weights that the codes stand for, in fp32 (exact) */
+int nerf_dequantize_w4(const unsigned char* d_codes, const unsigned short* d_scales, int rows, int cols, int group,
+                       float* d_dst, long ld_dst);
+/* Y[M][N] = act(X[M][K] W[N][K]^T) for W in 4 bits: x_type and y_type NERF_TYPE_*, rows ldx >= K and ldy >= N elements
+ * apart, epilogue 0: act is nothing, 1: swish.  Products are exact, sums are in fp32 and Y is rounded once.  Made for
+ * few rows (one to some dozens); for hundreds, dequantize once and use nerf_gemm_f32 or nerf_gemm_bf16_nt.  Needs
+ * d_codes 16-byte aligned.  d_workspace: nerf_gemm_w4_workspace bytes, 16-byte aligned (may be NULL where that is 0);
+ * calls that overlap in time need one each. */
+size_t nerf_gemm_w4_workspace(int M, int N, int K);
+int nerf_gemm_w4(const void* d_X, int x_type, long ldx, const unsigned char* d_codes, const unsigned short* d_scales,
+                 int group, void* d_Y, int y_type, long ldy, int M, int N, int K, int epilogue, void* d_workspace,
+                 size_t workspace_bytes);
+
 /* ---- dataset on the device -------------------------------------------------------------------- */
 typedef struct NerfDeviceDataset NerfDeviceDataset;
 /* copies every camera and every image's RGBA8 pixels of a Dataset (data.h:25-29) to the device */

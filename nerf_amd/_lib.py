@@ -135,6 +135,13 @@ _SIGS = {
     "nerf_adamw_step": (C.c_int, [VP, C.c_int, C.c_float, C.c_float, VP, C.c_float, C.c_ulonglong]),
     "nerf_adamw_read_states": (C.c_int, [VP, VP, VP]),
     "nerf_grad_norm": (C.c_int, [VP, C.c_float, VP]),
+    # weights in 4 bits
+    "nerf_w4_row_bytes": (C.c_size_t, [C.c_int]),
+    "nerf_quantize_w4": (C.c_int, [VP, C.c_long, C.c_int, C.c_int, C.c_int, VP, VP]),
+    "nerf_dequantize_w4": (C.c_int, [VP, VP, C.c_int, C.c_int, C.c_int, VP, C.c_long]),
+    "nerf_gemm_w4_workspace": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
+    "nerf_gemm_w4": (C.c_int, [VP, C.c_int, C.c_long, VP, VP, C.c_int, VP, C.c_int, C.c_long, C.c_int, C.c_int, C.c_int,
+                               C.c_int, VP, C.c_size_t]),
     # dataset / encode
     "nerf_dataset_upload": (VP, [C.POINTER(Dataset)]),
     "nerf_dataset_upload_cameras": (VP, [C.POINTER(Dataset)]),
