@@ -446,7 +446,7 @@ static int build_plan(const NerfAdamwTensor* tensors, int count, int state_bits,
         plan->bytes += (double)s.n * (8.0 + g_item + (state_bits == 8 ? 4.0 : 16.0) + (s.w_bf16 ? 2.0 : 0.0));
         first += s.n;
         const size_t pieces = s.n / plan->chunk + (s.n % plan->chunk != 0);
-        if (chunks.size() + pieces > 0x7fffffffu) return NERF_ERR_ARG;
+        if (chunks.size() + pieces > 0xffffffu) return NERF_ERR_ARG;  // a launch has fewer than 2^32 threads
         for (size_t p = 0; p < pieces; p++) chunks.push_back(Chunk{(unsigned)k, (unsigned)p});
     }
     plan->chunks = (unsigned)chunks.size();

@@ -117,9 +117,6 @@ struct W4Args {
     int M, N, K, group, groups, x_bf16, y_bf16, epilogue;
 };
 
-__device__ __forceinline__ float load_x(const W4Args& a, long at) {
-    return a.x_bf16 ? bf16_to_f32(((const unsigned short*)a.X)[at]) : ((const float*)a.X)[at];
-}
 __device__ __forceinline__ void store_y(const W4Args& a, long at, float y) {
     // sigmoid through the hardware exp2 and reciprocal, as in the other products' epilogues
     if (a.epilogue == 1) y = y * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(y * -1.44269504088896340736f));
@@ -127,32 +124,239 @@ __device__ __forceinline__ void store_y(const W4Args& a, long at, float y) {
     else ((float*)a.Y)[at] = y;
 }
 
-// One wavefront per (row of W, row of X): a lane takes every 64th unit.
-__global__ __launch_bounds__(256) void gemv_w4_kernel(const W4Args a) {
-    const int lane = threadIdx.x & 63;
-    const long n = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (n >= a.N) return;
-    const int m = blockIdx.y;
-    const int units = (a.K + 31) / 32;
-    float acc = 0.0f;
-    for (int u = lane; u < units; u += 64) {
-        const u32x4 c = *reinterpret_cast<const u32x4*>(a.codes + n * a.row_bytes + (long)u * 16);
-        const float scale = bf16_to_f32(a.scales[n * a.groups + u * 32 / a.group]);
-        float part = 0.0f;
+// One product for any number of rows: a workgroup takes 16 NT columns of Y (rows of W) and 16 MT rows of X; its
+// wavefronts share out the contraction in chunks of 128 columns and add up in LDS at the end, so no piece of W or X is
+// read twice in a workgroup.  Per chunk a lane loads 16 bytes (one unit of 32 columns) of one of 16 rows of W; four
+// lane swaps turn the four units that four lanes hold of a row into the four steps of a matrix instruction
+// (16 x 16 x 32, both operands bf16), so that a step's 32 columns lie in one group and its sum takes one scale.
+//   Codes are bf16 numbers exactly.  An fp32 x goes as three bf16 numbers that add up to it exactly (its upper, middle
+// and lower 8 significant bits, cut off), with one instruction each: products are exact, sums are fp32.
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x2u __attribute__((ext_vector_type(2), aligned(2)));
+typedef unsigned u32u __attribute__((aligned(2)));
+typedef unsigned u32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned u32x4u2 __attribute__((ext_vector_type(4), aligned(2)));
+
+// eight codes as eight bf16
+__device__ __forceinline__ bf16x8 values8_bf16(unsigned c) {
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, 1.0f, 1);
+    const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, 1.0f, 2), e = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, 1.0f, 3);
+    return bf16x8{a[0], a[1], b[0], b[1], d[0], d[1], e[0], e[1]};
+}
+
+// upper halves of two words, the first one below
+__device__ __forceinline__ unsigned upper_halves(unsigned lo, unsigned hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302); }
+
+// what eight consecutive values of X are as matrix operands
+template <bool XBF>
+struct Operand;
+template <>
+struct Operand<true> {
+    static constexpr int PARTS = 1;
+    u32x4 p[1];
+};
+template <>
+struct Operand<false> {
+    static constexpr int PARTS = 3;
+    u32x4 p[3];
+};
+
+template <bool XBF>
+struct Raw {  // as loaded
+    u32x4 a, b;  // eight fp32; bf16: a alone
+};
+
+template <bool XBF>
+__device__ __forceinline__ Raw<XBF> load_raw(const void* row, int col, int K, bool whole) {
+    Raw<XBF> r = {};
+    if (XBF) {
+        const unsigned short* p = (const unsigned short*)row + col;
+        if (whole) r.a = *reinterpret_cast<const u32x4u2*>(p);
+        else
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-            float v[8];
-            values8(c[q], v);
-            for (int k = 0; k < 8; k++) {
-                const int col = u * 32 + q * 8 + k;
-                if (col < a.K) part = __builtin_fmaf(load_x(a, (long)m * a.ldx + col), v[k], part);
+            for (int k = 0; k < 8; k++)
+                if (col + k < K) r.a[k / 2] |= (unsigned)p[k] << (16 * (k & 1));
+    } else {
+        const unsigned* p = (const unsigned*)row + col;
+        if (whole) {
+            r.a = *reinterpret_cast<const u32x4u*>(p);
+            r.b = *reinterpret_cast<const u32x4u*>(p + 4);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                if (col + k < K) r.a[k] = p[k];
+                if (col + 4 + k < K) r.b[k] = p[k + 4];
             }
         }
-        acc = __builtin_fmaf(part, scale, acc);
+    }
+    return r;
+}
+
+template <bool XBF>
+__device__ __forceinline__ void split(const Raw<XBF>& r, Operand<XBF>& o) {
+    if constexpr (XBF) {
+        o.p[0] = r.a;
+    } else {
+        unsigned hi[8], mid[8], lo[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const unsigned x = k < 4 ? r.a[k] : r.b[k - 4];
+            hi[k] = x & 0xFFFF0000u;
+            // infinity less itself would be NaN: what is not finite goes in the first part alone
+            const float rest = __builtin_bit_cast(float, x) - __builtin_bit_cast(float, hi[k]);
+            const unsigned m = (x & 0x7F800000u) == 0x7F800000u ? 0u : __builtin_bit_cast(unsigned, rest);
+            mid[k] = m & 0xFFFF0000u;
+            lo[k] = __builtin_bit_cast(unsigned, __builtin_bit_cast(float, m) - __builtin_bit_cast(float, mid[k]));
+            // a NaN whose upper half alone would read as infinity stays a NaN
+            if ((x & 0x7FFFFFFFu) > 0x7F800000u) hi[k] = 0x7FC00000u;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            o.p[0][k] = upper_halves(hi[2 * k], hi[2 * k + 1]);
+            o.p[1][k] = upper_halves(mid[2 * k], mid[2 * k + 1]);
+            o.p[2][k] = upper_halves(lo[2 * k], lo[2 * k + 1]);
+        }
+    }
+}
+
+// d[s] of lane group j (16 lanes each) becomes what d[j] of lane group s was
+__device__ __forceinline__ void transpose4(u32x4& d) {
+    auto a = __builtin_amdgcn_permlane32_swap(d[0], d[2], false, false);
+    auto b = __builtin_amdgcn_permlane32_swap(d[1], d[3], false, false);
+    auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
+    auto e = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+    d = u32x4{c[0], c[1], e[0], e[1]};
+}
+
+template <int GROUP>
+__device__ __forceinline__ void load_scales(const unsigned short* row, int chunk, int K, bool whole, float* s) {
+    const int first = chunk * 128 / GROUP;
+    if (whole) {
+        if (GROUP == 32) {
+            const u32x2u w = *reinterpret_cast<const u32x2u*>(row + first);
+            s[0] = __builtin_bit_cast(float, w[0] << 16);
+            s[1] = __builtin_bit_cast(float, w[0] & 0xFFFF0000u);
+            s[2] = __builtin_bit_cast(float, w[1] << 16);
+            s[3] = __builtin_bit_cast(float, w[1] & 0xFFFF0000u);
+        } else if (GROUP == 64) {
+            const unsigned w = *reinterpret_cast<const u32u*>(row + first);
+            s[0] = s[1] = __builtin_bit_cast(float, w << 16);
+            s[2] = s[3] = __builtin_bit_cast(float, w & 0xFFFF0000u);
+        } else {
+            s[0] = s[1] = s[2] = s[3] = bf16_to_f32(row[first]);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++) s[k] = chunk * 128 + 32 * k < K ? bf16_to_f32(row[(chunk * 128 + 32 * k) / GROUP]) : 0.0f;
+    }
+}
+
+template <int MT, int NT, bool XBF, int GROUP>
+__global__ __launch_bounds__(512) void gemm_w4_kernel(const W4Args a) {
+    extern __shared__ __attribute__((aligned(16))) f32x4 sums[];  // [wavefronts][NT][64]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const int ln = lane & 15, lj = lane >> 4;
+    const long n0 = (long)blockIdx.x * (16 * NT);
+    const long m0 = (long)blockIdx.y * (16 * MT);
+    const unsigned char* wrow[NT];
+    const unsigned short* srow[NT];
+    const char* xrow[MT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {  // rows past the end repeat the last one; what they give is not stored
+        const long n = min(n0 + t * 16 + ln, (long)a.N - 1);
+        wrow[t] = a.codes + n * a.row_bytes + lj * 16;
+        srow[t] = a.scales + n * a.groups;
     }
 #pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) acc += __shfl_xor(acc, d, 64);
-    if (lane == 0) store_y(a, (long)m * a.ldy + n, acc);
+    for (int t = 0; t < MT; t++)
+        xrow[t] = (const char*)a.X + min(m0 + t * 16 + ln, (long)a.M - 1) * a.ldx * (XBF ? 2 : 4);
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int t = 0; t < NT; t++) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int chunks = (a.K + 127) / 128, units = (a.K + 31) / 32;
+    for (int c = wave; c < chunks; c += waves) {
+        const bool whole = c * 128 + 128 <= a.K;
+        u32x4 d[NT];
+        float scale[NT][4];
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            d[t] = u32x4{0, 0, 0, 0};
+            if (whole || c * 4 + lj < units) d[t] = *reinterpret_cast<const u32x4*>(wrow[t] + (long)c * 64);
+            load_scales<GROUP>(srow[t], c, a.K, whole, scale[t]);
+        }
+        Raw<XBF> raw[MT][4];
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int s = 0; s < 4; s++) raw[i][s] = load_raw<XBF>(xrow[i], c * 128 + 32 * s + 8 * lj, a.K, whole);
+#pragma unroll
+        for (int t = 0; t < NT; t++) transpose4(d[t]);
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+            Operand<XBF> x[MT];
+#pragma unroll
+            for (int i = 0; i < MT; i++) split<XBF>(raw[i][s], x[i]);
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const bf16x8 w = values8_bf16(d[t][s]);
+#pragma unroll
+                for (int i = 0; i < MT; i++) {
+                    f32x4 part = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int q = Operand<XBF>::PARTS - 1; q >= 0; q--)
+                        part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x[i].p[q]), w, part, 0, 0, 0);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) acc[i][t][r] = __builtin_fmaf(part[r], scale[t][s], acc[i][t][r]);
+                }
+            }
+        }
+    }
+    // lane (ln, lj) holds column ln, rows 4 lj .. 4 lj + 3 of each 16 x 16 tile
+#pragma unroll
+    for (int i = 0; i < MT; i++) {
+        if (i) __syncthreads();
+#pragma unroll
+        for (int t = 0; t < NT; t++) sums[(wave * NT + t) * 64 + lane] = acc[i][t];
+        __syncthreads();
+        for (int e = threadIdx.x; e < NT * 64; e += blockDim.x) {
+            f32x4 y = sums[e];
+            for (int w = 1; w < waves; w++) {
+                const f32x4 z = sums[w * NT * 64 + e];
+#pragma unroll
+                for (int r = 0; r < 4; r++) y[r] += z[r];
+            }
+            const long n = n0 + (e >> 6) * 16 + (e & 15);
+            const long m = m0 + i * 16 + ((e & 63) >> 4) * 4;
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                if (n < a.N && m + r < a.M) store_y(a, (m + r) * a.ldy + n, y[r]);
+        }
+    }
+}
+
+template <int MT, int NT, bool XBF, int GROUP>
+void launch_gemm(const W4Args& a) {
+    const int chunks = (a.K + 127) / 128;
+    int waves = 8;
+    while (waves > 1 && waves / 2 >= chunks) waves /= 2;
+    hipLaunchKernelGGL((gemm_w4_kernel<MT, NT, XBF, GROUP>),
+                       dim3((unsigned)((a.N + 16L * NT - 1) / (16 * NT)), (unsigned)((a.M + 16L * MT - 1) / (16 * MT))),
+                       dim3(64 * waves), waves * NT * 64 * sizeof(f32x4), stream(), a);
+}
+template <int MT, int NT>
+void launch_gemm(const W4Args& a) {
+    if (a.x_bf16) {
+        if (a.group == 32) launch_gemm<MT, NT, true, 32>(a);
+        else if (a.group == 64) launch_gemm<MT, NT, true, 64>(a);
+        else launch_gemm<MT, NT, true, 128>(a);
+    } else {
+        if (a.group == 32) launch_gemm<MT, NT, false, 32>(a);
+        else if (a.group == 64) launch_gemm<MT, NT, false, 64>(a);
+        else launch_gemm<MT, NT, false, 128>(a);
+    }
 }
 
 bool group_ok(int group) { return group == 32 || group == 64 || group == 128; }
@@ -226,9 +430,15 @@ int nerf_gemm_w4(const void* d_X, int x_type, long ldx, const unsigned char* d_c
     a.ldx = ldx; a.ldy = ldy; a.row_bytes = (long)nerf_w4_row_bytes(K);
     a.M = M; a.N = N; a.K = K; a.group = group; a.groups = ceil_div(K, group);
     a.x_bf16 = x_type == NERF_TYPE_BF16; a.y_bf16 = y_type == NERF_TYPE_BF16; a.epilogue = epilogue;
-    if (M > 65535) return NERF_ERR_ARG;
     ProfScope prof(K_GEMM_W4, 2.0 * M * N * K);
-    hipLaunchKernelGGL(gemv_w4_kernel, dim3((unsigned)ceil_div(N, 4), (unsigned)M), dim3(256), 0, stream(), a);
+    if (M <= 16) {
+        if (N >= 8192) launch_gemm<1, 4>(a);
+        else launch_gemm<1, 1>(a);
+    } else if (M <= 32) {
+        launch_gemm<2, 2>(a);
+    } else {
+        launch_gemm<4, 2>(a);
+    }
     return hipGetLastError() == hipSuccess ? NERF_OK : NERF_ERR_HIP;
 }
 
