@@ -7,6 +7,7 @@
 #include "../../include/nerf_amd.h"
 
 #include <algorithm>
+#include <type_traits>
 
 #pragma clang fp contract(off)
 
@@ -108,6 +109,15 @@ __global__ __launch_bounds__(256) void dequantize_w4_kernel(const unsigned char*
 }
 
 // ---- products -------------------------------------------------------------------------------------------
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x2u __attribute__((ext_vector_type(2), aligned(2)));
+typedef unsigned u32u __attribute__((aligned(2)));
+typedef unsigned u32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned u32x4u2 __attribute__((ext_vector_type(4), aligned(2)));
+
+constexpr int WAVES = 8;  // of a workgroup
+
 struct W4Args {
     const void* X;
     const unsigned char* codes;
@@ -124,20 +134,207 @@ __device__ __forceinline__ void store_y(const W4Args& a, long at, float y) {
     else ((float*)a.Y)[at] = y;
 }
 
-// One product for any number of rows: a workgroup takes 16 NT columns of Y (rows of W) and 16 MT rows of X; its
-// wavefronts share out the contraction in chunks of 128 columns and add up in LDS at the end, so no piece of W or X is
-// read twice in a workgroup.  Per chunk a lane loads 16 bytes (one unit of 32 columns) of one of 16 rows of W; four
-// lane swaps turn the four units that four lanes hold of a row into the four steps of a matrix instruction
-// (16 x 16 x 32, both operands bf16), so that a step's 32 columns lie in one group and its sum takes one scale.
-//   Codes are bf16 numbers exactly.  An fp32 x goes as three bf16 numbers that add up to it exactly (its upper, middle
-// and lower 8 significant bits, cut off), with one instruction each: products are exact, sums are fp32.
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef unsigned u32x2u __attribute__((ext_vector_type(2), aligned(2)));
-typedef unsigned u32u __attribute__((aligned(2)));
-typedef unsigned u32x4u __attribute__((ext_vector_type(4), aligned(4)));
-typedef unsigned u32x4u2 __attribute__((ext_vector_type(4), aligned(2)));
+// ---- one or two rows ------------------------------------------------------------------------------------
+// A lane keeps the X of one unit (32 columns) of each row in registers as fp32 and walks down the rows of W: 16 bytes of
+// codes and a scale per row, converted two at a time and multiplied by fused multiply-adds.  Sixty-four lanes are 2048
+// columns: `kw` wavefronts lie side by side along K (a longer K takes several rounds), a shorter K has `lanes` lanes to
+// a row and several rows to a wavefront.  B loads of W are on their way while the B before are worked on.
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float x) {
+    const int y = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true);
+    return x + __builtin_bit_cast(float, y);
+}
+// a + b where the lower half of the result is the sum of a's halves and the upper half that of b's; and for every two
+// rows of sixteen lanes alike
+__device__ __forceinline__ float fold32(float a, float b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
+    const unsigned lo = r[0], hi = r[1];  // (a bit cast of r[1] itself reads r[0])
+    return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+}
+__device__ __forceinline__ float fold16(float a, float b) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
+    const unsigned lo = r[0], hi = r[1];  // (a bit cast of r[1] itself reads r[0])
+    return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+}
+__device__ __forceinline__ float sum16(float x) {
+    return add_dpp<0x140>(add_dpp<0x141>(add_dpp<0x4E>(add_dpp<0xB1>(x))));
+}
 
+constexpr int GEMV_LOADS = 2;  // of W on their way, and as many worked on
+
+struct GemvShape {
+    int log_lanes;  // 2^log_lanes lanes to a row: 64, or less where that is all of K
+    int log_kw;     // 2^log_kw wavefronts along K (of WAVES)
+    int loads;      // of W per wavefront and round, a multiple of B
+    int stride;     // bytes between a unit's pieces of an fp32 X in LDS: 128 past a multiple of 256
+};
+
+template <int M, bool XBF>
+__global__ __launch_bounds__(64 * WAVES) void gemv_w4_kernel(const W4Args a, const GemvShape g) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    constexpr int B = GEMV_LOADS;
+    // LDS: an fp32 X as [row][piece of four columns in a unit][unit], so that it is read from memory and from LDS in runs
+    // (a lane's unit is 128 bytes, and as many lines as lanes are slow to look up; a bf16 unit is half of that and is
+    // read directly); then the sums [M][kw][rows of the workgroup]
+    float* sums = reinterpret_cast<float*>(lds + (XBF ? 0 : M * 8 * g.stride));
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lanes = 1 << g.log_lanes, kw = 1 << g.log_kw;
+    const int wk = wave & (kw - 1), wn = wave >> g.log_kw;
+    const int at_once = 64 >> g.log_lanes;       // rows of a load
+    const int wave_rows = g.loads * at_once, block_rows = wave_rows * (WAVES >> g.log_kw);
+    const int sub = lane >> g.log_lanes;         // the lane's row of a load
+    const int units = (a.K + 31) / 32, shift = a.group == 32 ? 0 : a.group == 64 ? 1 : 2;
+    const long n0 = (long)blockIdx.x * block_rows + wn * wave_rows;
+    for (int round = 0; round * kw * 64 < units; round++) {
+        const int unit = (round * kw + wk) * 64 + (lane & (lanes - 1));
+        const bool live = unit < units;
+        const int held = min(unit, units - 1);
+        const unsigned char* codes = a.codes + (long)held * 16;
+        const unsigned short* scales = a.scales + (held >> shift);
+        u32x4 next[B];
+        unsigned short next_scale[B];
+        auto load = [&](int first) {
+#pragma unroll
+            for (int b = 0; b < B; b++) {  // rows past the end repeat the last one; what they give is not stored
+                const long n = min(n0 + (first + b) * at_once + sub, (long)a.N - 1);
+                next[b] = *reinterpret_cast<const u32x4*>(codes + n * a.row_bytes);
+                next_scale[b] = scales[n * a.groups];
+            }
+        };
+        load(0);
+        float x[M][32];
+        if constexpr (XBF) {
+#pragma unroll
+            for (int m = 0; m < M; m++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const int col = unit * 32 + q * 8;
+                    const unsigned short* from = (const unsigned short*)a.X + m * a.ldx + col;
+                    u32x4 v = {0, 0, 0, 0};
+                    if (col + 8 <= a.K) v = *reinterpret_cast<const u32x4u2*>(from);
+                    else if (col < a.K)
+#pragma unroll
+                        for (int k = 0; k < 7; k++)
+                            if (col + k < a.K) v[k / 2] |= (unsigned)from[k] << (16 * (k & 1));
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const unsigned word = v[e];
+                        x[m][q * 8 + 2 * e] = __builtin_bit_cast(float, word << 16);
+                        x[m][q * 8 + 2 * e + 1] = __builtin_bit_cast(float, word & 0xFFFF0000u);
+                    }
+                }
+        } else {
+            if (round) __syncthreads();
+            const int width = kw << g.log_lanes, base = round * kw * 64;  // units of a round, and the first one
+            for (int p = threadIdx.x; p < M * width * 8; p += 64 * WAVES) {
+                const int m = M == 1 ? 0 : p >= width * 8, at = p - m * width * 8;
+                const int col = base * 32 + at * 4;
+                const float* from = (const float*)a.X + m * a.ldx + col;
+                f32x4 v = {0.f, 0.f, 0.f, 0.f};
+                if (col + 4 <= a.K) v = *reinterpret_cast<const f32x4u*>(from);
+                else
+                    for (int k = 0; k < 3; k++)
+                        if (col + k < a.K) v[k] = from[k];
+                *reinterpret_cast<f32x4*>(lds + (m * 8 + at % 8) * g.stride + at / 8 * 16) = v;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int m = 0; m < M; m++)
+#pragma unroll
+                for (int q = 0; q < 8; q++) {
+                    const f32x4 v = *reinterpret_cast<const f32x4*>(lds + (m * 8 + q) * g.stride + (unit - base) * 16);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[m][q * 4 + e] = v[e];
+                }
+        }
+        for (int first = 0; first < g.loads; first += B) {
+            u32x4 c[B];
+            float scale[B], y[M][B];
+#pragma unroll
+            for (int b = 0; b < B; b++) {
+                c[b] = next[b];
+                scale[b] = live ? bf16_to_f32(next_scale[b]) : 0.0f;
+            }
+            if (first + B < g.loads) load(first + B);
+            asm volatile("" ::: "memory");  // the loads stay here, B rows ahead of their use
+#pragma unroll
+            for (int b = 0; b < B; b++) {
+                float part[M];
+#pragma unroll
+                for (int m = 0; m < M; m++) part[m] = 0.0f;
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    float v[8];
+                    values8(c[b][q], v);
+#pragma unroll
+                    for (int m = 0; m < M; m++)
+#pragma unroll
+                        for (int k = 0; k < 8; k++) part[m] = __builtin_fmaf(x[m][q * 8 + k], v[k], part[m]);
+                }
+#pragma unroll
+                for (int m = 0; m < M; m++) y[m][b] = part[m] * scale[b];
+            }
+            // sums over a row's lanes, and who holds which row of this turn
+            int row = first * at_once + sub, count = B;
+            bool writes = (lane & (lanes - 1)) == 0;
+            if (g.log_lanes == 6) {
+#pragma unroll
+                for (int m = 0; m < M; m++) {  // two rows go to the two halves
+                    const float z = fold32(y[m][0], y[m][1]);
+                    y[m][0] = sum16(fold16(z, z));
+                }
+                row = first + (lane >> 5);
+                writes = (lane & 31) == 0;
+                count = 1;
+            } else {
+#pragma unroll
+                for (int m = 0; m < M; m++)
+#pragma unroll
+                    for (int b = 0; b < B; b++) {
+                        float t = y[m][b];
+                        if (g.log_lanes > 0) t = add_dpp<0xB1>(t);
+                        if (g.log_lanes > 1) t = add_dpp<0x4E>(t);
+                        if (g.log_lanes > 2) t = add_dpp<0x141>(t);
+                        if (g.log_lanes > 3) t = add_dpp<0x140>(t);
+                        if (g.log_lanes > 4) t = fold16(t, t);
+                        y[m][b] = t;
+                    }
+            }
+            if (writes) {
+#pragma unroll
+                for (int m = 0; m < M; m++) {
+                    float* to = sums + (m * kw + wk) * block_rows + wn * wave_rows + row;
+#pragma unroll
+                    for (int b = 0; b < B; b++)
+                        if (b < count) to[b * at_once] = round ? to[b * at_once] + y[m][b] : y[m][b];
+                }
+            }
+        }
+    }
+    __syncthreads();
+    for (int r = threadIdx.x; r < block_rows * M; r += 64 * WAVES) {
+        const int m = r / block_rows, row = r - m * block_rows;
+        const long n = (long)blockIdx.x * block_rows + row;
+        if (n >= a.N) continue;
+        float y = 0.0f;
+        for (int k = 0; k < kw; k++) y += sums[(m * kw + k) * block_rows + row];
+        store_y(a, m * a.ldy + n, y);
+    }
+}
+
+// ---- many rows ------------------------------------------------------------------------------------------
+// One product for any number of rows.  A workgroup of eight wavefronts takes R MT rows of X and 16 NT columns of Y (rows
+// of W) for each of `8 / kw` wavefronts; `kw` wavefronts share the same columns and split the contraction, which goes in
+// chunks of 128 columns.
+//   X: a slice of the rows' columns is put in LDS as matrix operands, once for all wavefronts: bf16 as it is, fp32 as
+// three bf16 numbers that add up to it exactly (its upper, middle and lower 8 significant bits, cut off), with one matrix
+// instruction each.  Codes are bf16 numbers exactly, so products are exact and sums are fp32.  The next slice is on its
+// way in registers while one is worked on.
+//   W: per chunk a lane loads 16 bytes (one unit of 32 columns) of one of 16 rows straight to registers, DEPTH chunks
+// ahead; four lane swaps turn the four units that four lanes hold of a row into the four steps of a matrix instruction
+// (16 x 16 x 32), so that a step's 32 columns lie in one group and the sum over a group takes one scale.  Columns of
+// workgroups start at different chunks of a slice: rows of W are often a power of two apart, and workgroups that walk
+// them in step would all ask the same few memory channels.
 // eight codes as eight bf16
 __device__ __forceinline__ bf16x8 values8_bf16(unsigned c) {
     const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, 1.0f, 1);
@@ -148,215 +345,383 @@ __device__ __forceinline__ bf16x8 values8_bf16(unsigned c) {
 // upper halves of two words, the first one below
 __device__ __forceinline__ unsigned upper_halves(unsigned lo, unsigned hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302); }
 
-// what eight consecutive values of X are as matrix operands
-template <bool XBF>
-struct Operand;
-template <>
-struct Operand<true> {
-    static constexpr int PARTS = 1;
-    u32x4 p[1];
-};
-template <>
-struct Operand<false> {
-    static constexpr int PARTS = 3;
-    u32x4 p[3];
-};
+// the upper, middle and lower 8 significant bits of an fp32 number, each as the upper half of a word (a bf16 number)
+__device__ __forceinline__ void split3(unsigned x, unsigned& hi, unsigned& mid, unsigned& lo) {
+    // infinity less itself would be NaN: what is not finite goes in the first part alone
+    const bool special = (x & 0x7F800000u) == 0x7F800000u;
+    const float rest = special ? 0.0f : __builtin_bit_cast(float, x) - __builtin_bit_cast(float, x & 0xFFFF0000u);
+    mid = __builtin_bit_cast(unsigned, rest);
+    lo = __builtin_bit_cast(unsigned, rest - __builtin_bit_cast(float, mid & 0xFFFF0000u));
+    // a NaN whose upper half alone would read as infinity stays a NaN
+    hi = (x & 0x7FFFFFFFu) > 0x7F800000u ? 0x7FC00000u : x;
+}
 
+// Eight consecutive values of a row of X as they lie in memory, and as one or three operands of eight bf16
 template <bool XBF>
-struct Raw {  // as loaded
-    u32x4 a, b;  // eight fp32; bf16: a alone
-};
+struct Piece {
+    u32x4 v[XBF ? 1 : 2];
 
-template <bool XBF>
-__device__ __forceinline__ Raw<XBF> load_raw(const void* row, int col, int K, bool whole) {
-    Raw<XBF> r = {};
-    if (XBF) {
-        const unsigned short* p = (const unsigned short*)row + col;
-        if (whole) r.a = *reinterpret_cast<const u32x4u2*>(p);
-        else
-#pragma unroll
-            for (int k = 0; k < 8; k++)
-                if (col + k < K) r.a[k / 2] |= (unsigned)p[k] << (16 * (k & 1));
-    } else {
-        const unsigned* p = (const unsigned*)row + col;
-        if (whole) {
-            r.a = *reinterpret_cast<const u32x4u*>(p);
-            r.b = *reinterpret_cast<const u32x4u*>(p + 4);
+    __device__ __forceinline__ void load(const void* row, int col) {
+        if constexpr (XBF) {
+            v[0] = *reinterpret_cast<const u32x4u2*>((const unsigned short*)row + col);
         } else {
+            v[0] = *reinterpret_cast<const u32x4u*>((const unsigned*)row + col);
+            v[1] = *reinterpret_cast<const u32x4u*>((const unsigned*)row + col + 4);
+        }
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int k = 0; k < (XBF ? 1 : 2); k++) v[k] = u32x4{0, 0, 0, 0};
+    }
+    __device__ __forceinline__ void operands(u32x4* o) const {
+        if constexpr (XBF) {
+            o[0] = v[0];
+        } else {
+            unsigned hi[8], mid[8], lo[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) split3(v[k / 4][k % 4], hi[k], mid[k], lo[k]);
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                if (col + k < K) r.a[k] = p[k];
-                if (col + 4 + k < K) r.b[k] = p[k + 4];
+                o[0][k] = upper_halves(hi[2 * k], hi[2 * k + 1]);
+                o[1][k] = upper_halves(mid[2 * k], mid[2 * k + 1]);
+                o[2][k] = upper_halves(lo[2 * k], lo[2 * k + 1]);
             }
         }
     }
-    return r;
-}
-
-template <bool XBF>
-__device__ __forceinline__ void split(const Raw<XBF>& r, Operand<XBF>& o) {
-    if constexpr (XBF) {
-        o.p[0] = r.a;
-    } else {
-        unsigned hi[8], mid[8], lo[8];
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-            const unsigned x = k < 4 ? r.a[k] : r.b[k - 4];
-            hi[k] = x & 0xFFFF0000u;
-            // infinity less itself would be NaN: what is not finite goes in the first part alone
-            const float rest = __builtin_bit_cast(float, x) - __builtin_bit_cast(float, hi[k]);
-            const unsigned m = (x & 0x7F800000u) == 0x7F800000u ? 0u : __builtin_bit_cast(unsigned, rest);
-            mid[k] = m & 0xFFFF0000u;
-            lo[k] = __builtin_bit_cast(unsigned, __builtin_bit_cast(float, m) - __builtin_bit_cast(float, mid[k]));
-            // a NaN whose upper half alone would read as infinity stays a NaN
-            if ((x & 0x7FFFFFFFu) > 0x7F800000u) hi[k] = 0x7FC00000u;
-        }
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            o.p[0][k] = upper_halves(hi[2 * k], hi[2 * k + 1]);
-            o.p[1][k] = upper_halves(mid[2 * k], mid[2 * k + 1]);
-            o.p[2][k] = upper_halves(lo[2 * k], lo[2 * k + 1]);
-        }
-    }
-}
+};
 
 // d[s] of lane group j (16 lanes each) becomes what d[j] of lane group s was
-__device__ __forceinline__ void transpose4(u32x4& d) {
+__device__ __forceinline__ u32x4 transpose4(u32x4 d) {
     auto a = __builtin_amdgcn_permlane32_swap(d[0], d[2], false, false);
     auto b = __builtin_amdgcn_permlane32_swap(d[1], d[3], false, false);
     auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
     auto e = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
-    d = u32x4{c[0], c[1], e[0], e[1]};
+    return u32x4{c[0], c[1], e[0], e[1]};
 }
 
+// A chunk of one of a lane's rows of W: its codes, and the scales of the chunk's groups as they lie in memory.  In the last
+// chunk of a row that is no multiple of 128 long, a unit past the row's end is the last one again (X is zero there), and
+// a group past the end has the scale zero.
 template <int GROUP>
-__device__ __forceinline__ void load_scales(const unsigned short* row, int chunk, int K, bool whole, float* s) {
-    const int first = chunk * 128 / GROUP;
-    if (whole) {
-        if (GROUP == 32) {
-            const u32x2u w = *reinterpret_cast<const u32x2u*>(row + first);
-            s[0] = __builtin_bit_cast(float, w[0] << 16);
-            s[1] = __builtin_bit_cast(float, w[0] & 0xFFFF0000u);
-            s[2] = __builtin_bit_cast(float, w[1] << 16);
-            s[3] = __builtin_bit_cast(float, w[1] & 0xFFFF0000u);
-        } else if (GROUP == 64) {
-            const unsigned w = *reinterpret_cast<const u32u*>(row + first);
-            s[0] = s[1] = __builtin_bit_cast(float, w << 16);
-            s[2] = s[3] = __builtin_bit_cast(float, w & 0xFFFF0000u);
-        } else {
-            s[0] = s[1] = s[2] = s[3] = bf16_to_f32(row[first]);
-        }
-    } else {
-#pragma unroll
-        for (int k = 0; k < 4; k++) s[k] = chunk * 128 + 32 * k < K ? bf16_to_f32(row[(chunk * 128 + 32 * k) / GROUP]) : 0.0f;
-    }
-}
+struct Chunk4 {
+    static constexpr int GROUPS = 128 / GROUP;
+    u32x4 codes;
+    unsigned scales[GROUP == 32 ? 2 : 1];
 
-template <int MT, int NT, bool XBF, int GROUP>
-__global__ __launch_bounds__(512) void gemm_w4_kernel(const W4Args a) {
-    extern __shared__ __attribute__((aligned(16))) f32x4 sums[];  // [wavefronts][NT][64]
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    // unit: of the lane, in a row of `units`; first: the chunk's first group, in a row of `groups`
+    __device__ __forceinline__ void load(const unsigned char* codes_row, const unsigned short* scales_row, int unit, int units, int first,
+                                         int groups) {
+        codes = *reinterpret_cast<const u32x4*>(codes_row + (long)min(unit, units - 1) * 16);
+        if (groups >= GROUPS) {
+            const int start = min(first, groups - GROUPS), past = (first - start) * 16;  // bits to drop
+            const unsigned short* p = scales_row + start;
+            if constexpr (GROUP == 32) {
+                const u32x2u s = *reinterpret_cast<const u32x2u*>(p);
+                const unsigned long long both = ((unsigned long long)s[1] << 32 | s[0]) >> past;
+                scales[0] = (unsigned)both;
+                scales[1] = (unsigned)(both >> 32);
+            } else if constexpr (GROUP == 64) {
+                scales[0] = *reinterpret_cast<const u32u*>(p) >> past;
+            } else {
+                scales[0] = *p;
+            }
+        } else {  // a row of one chunk with fewer groups
+            scales[0] = scales_row[0] | (groups > 1 ? (unsigned)scales_row[1] << 16 : 0u);
+            if constexpr (GROUP == 32) scales[1] = groups > 2 ? scales_row[2] : 0u;
+        }
+    }
+    __device__ __forceinline__ float scale(int g) const {  // of the chunk's group g
+        return __builtin_bit_cast(float, g & 1 ? scales[g / 2] & 0xFFFF0000u : scales[g / 2] << 16);
+    }
+};
+
+struct GemmShape {
+    int log_kw;        // 2^log_kw wavefronts split the contraction: 1, 2, 4 or 8
+    int split_chunks;  // chunks of one part of the contraction (gridDim.z parts), a multiple of a slice
+    float* partial;    // [parts][M][N], or null: one part, stored to Y
+};
+
+constexpr int DEPTH = 2;  // chunks of W on their way to a wavefront
+
+// chunks of a slice: with this many, a slice of R MT rows is four pieces of eight columns for each thread
+constexpr int slice_chunks(int r, int mt) { return 128 / (r * mt); }
+
+template <int R, int MT, int NT, bool XBF, int GROUP>
+__global__ __launch_bounds__(64 * WAVES) void gemm_w4_kernel(const W4Args a, const GemmShape g) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    constexpr int PARTS = XBF ? 1 : 3, STEPS = GROUP / 32, SLICE = slice_chunks(R, MT);
+    // LDS: [step of 32 columns][part][tile of R rows][unit of 8 columns][row], 16 bytes each: a wavefront reads an operand as
+    // one run; the steps are 16 bytes further apart, so that a run of a row's pieces is written to different banks
+    constexpr int TILE_BYTES = R * 64, PART_BYTES = MT * TILE_BYTES, STEP_BYTES = PARTS * PART_BYTES + 16;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ln = lane & 15, lj = lane >> 4;
-    const long n0 = (long)blockIdx.x * (16 * NT);
-    const long m0 = (long)blockIdx.y * (16 * MT);
+    const int kw = 1 << g.log_kw, columns = WAVES >> g.log_kw;  // wavefronts along the contraction, along N
+    const int wk = wave & (kw - 1), wn = wave >> g.log_kw;
+    const long n0 = ((long)blockIdx.x * columns + wn) * (16 * NT);
+    const long m0 = (long)blockIdx.y * (R * MT);
+    const int rows = (int)min((long)(R * MT), a.M - m0);
+    const int chunks = (a.K + 127) / 128, units = (a.K + 31) / 32;
+    const int first = blockIdx.z * g.split_chunks, end = min(chunks, first + g.split_chunks);
     const unsigned char* wrow[NT];
     const unsigned short* srow[NT];
-    const char* xrow[MT];
 #pragma unroll
     for (int t = 0; t < NT; t++) {  // rows past the end repeat the last one; what they give is not stored
         const long n = min(n0 + t * 16 + ln, (long)a.N - 1);
-        wrow[t] = a.codes + n * a.row_bytes + lj * 16;
+        wrow[t] = a.codes + n * a.row_bytes;
         srow[t] = a.scales + n * a.groups;
     }
+    // A wavefront's turns: SLICE / kw in each slice but the last, which has what is left.  Within a slice they begin at
+    // a place that differs from workgroup to workgroup.
+    const int log_turns = __builtin_ctz(SLICE) - g.log_kw;
+    const unsigned place = (blockIdx.x * 0x9E3779B1u) >> 16;
+    const int turns_all = end - first > wk ? (end - first - wk + kw - 1) >> g.log_kw : 0;
+    auto chunk_of = [&](int turn) {  // of turns_all
+        const int slice = turn >> log_turns, in_slice = turn - (slice << log_turns);
+        const int count = min(1 << log_turns, turns_all - (slice << log_turns));
+        int i = in_slice + (int)((place * (unsigned)count) >> 16);
+        if (i >= count) i -= count;
+        return first + slice * SLICE + wk + (i << g.log_kw);
+    };
+    auto load = [&](Chunk4<GROUP>* w, int turn) {
+        const int c = chunk_of(min(turn, turns_all - 1));  // past the end: the last one again
 #pragma unroll
-    for (int t = 0; t < MT; t++)
-        xrow[t] = (const char*)a.X + min(m0 + t * 16 + ln, (long)a.M - 1) * a.ldx * (XBF ? 2 : 4);
+        for (int t = 0; t < NT; t++) w[t].load(wrow[t], srow[t], c * 4 + lj, units, c * (128 / GROUP), a.groups);
+    };
     f32x4 acc[MT][NT];
 #pragma unroll
     for (int i = 0; i < MT; i++)
 #pragma unroll
         for (int t = 0; t < NT; t++) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int chunks = (a.K + 127) / 128, units = (a.K + 31) / 32;
-    for (int c = wave; c < chunks; c += waves) {
-        const bool whole = c * 128 + 128 <= a.K;
-        u32x4 d[NT];
-        float scale[NT][4];
+
+    // A thread's pieces of a slice: SLICE * 16 pieces in a row, R MT SLICE * 16 = 4 * 512 of them.  A piece that holds the
+    // row's last columns and others past them is put together by itself.
+    Piece<XBF> piece[4];
+    auto at_piece = [&](int r, int p) { return lds + (p / 4) * STEP_BYTES + (r / R) * TILE_BYTES + ((p % 4) * R + r % R) * 16; };
+    auto load_x = [&](int base) {
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            d[t] = u32x4{0, 0, 0, 0};
-            if (whole || c * 4 + lj < units) d[t] = *reinterpret_cast<const u32x4*>(wrow[t] + (long)c * 64);
-            load_scales<GROUP>(srow[t], c, a.K, whole, scale[t]);
+        for (int k = 0; k < 4; k++) {
+            const int q = threadIdx.x + k * 64 * WAVES, r = q / (SLICE * 16), col = base * 128 + q % (SLICE * 16) * 8;
+            piece[k].zero();
+            if (r < rows && col + 8 <= a.K) piece[k].load((const char*)a.X + (m0 + r) * a.ldx * (XBF ? 2 : 4), col);
         }
-        Raw<XBF> raw[MT][4];
+    };
+    auto stage_x = [&](int base) {
+        const int width = min(SLICE, end - base) * 16;  // pieces of a row that are looked at
 #pragma unroll
-        for (int i = 0; i < MT; i++)
+        for (int k = 0; k < 4; k++) {
+            const int q = threadIdx.x + k * 64 * WAVES, r = q / (SLICE * 16), p = q % (SLICE * 16), col = base * 128 + p * 8;
+            if (r < rows && p < width && (col + 8 <= a.K || col >= a.K)) {
+                u32x4 o[PARTS];
+                piece[k].operands(o);
+                char* at = at_piece(r, p);
 #pragma unroll
-            for (int s = 0; s < 4; s++) raw[i][s] = load_raw<XBF>(xrow[i], c * 128 + 32 * s + 8 * lj, a.K, whole);
+                for (int part = 0; part < PARTS; part++) *reinterpret_cast<u32x4*>(at + part * PART_BYTES) = o[part];
+            }
+        }
+        const int ragged = a.K / 8 * 8;
+        if (ragged != a.K && ragged >= base * 128 && ragged < (base + SLICE) * 128 && ragged < end * 128) {
+#pragma unroll 1
+            for (int q = threadIdx.x; q < rows * 8; q += 64 * WAVES) {
+                const int r = q / 8, col = ragged + q % 8;
+                unsigned h[3] = {0, 0, 0};
+                if (col < a.K) {
+                    const long from = (m0 + r) * a.ldx + col;
+                    if constexpr (XBF) h[0] = (unsigned)((const unsigned short*)a.X)[from] << 16;
+                    else split3(((const unsigned*)a.X)[from], h[0], h[1], h[2]);
+                }
+                char* at = at_piece(r, ragged / 8 - base * 16) + (q % 8) * 2;
 #pragma unroll
-        for (int t = 0; t < NT; t++) transpose4(d[t]);
+                for (int part = 0; part < PARTS; part++) *reinterpret_cast<unsigned short*>(at + part * PART_BYTES) = h[part] >> 16;
+            }
+        }
+    };
+    // rows past the end are read as what LDS holds there, or as the last row where R < 16: their sums are not stored
+    const char* xlane = lds + (lj * R + min(ln, R - 1)) * 16;
+
+    Chunk4<GROUP> w[DEPTH][NT];
+    if (turns_all) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; d++) load(w[d], d);
+    }
+    auto chunk = [&](const Chunk4<GROUP>* w, int turn, int base) {
+        const char* xs = xlane + (chunk_of(turn) - base) * (4 * STEP_BYTES);
+        u32x4 codes[NT];
+#pragma unroll
+        for (int t = 0; t < NT; t++) codes[t] = transpose4(w[t].codes);
+        f32x4 part[MT][NT];
 #pragma unroll
         for (int s = 0; s < 4; s++) {
-            Operand<XBF> x[MT];
+            bf16x8 x[MT][PARTS];
 #pragma unroll
-            for (int i = 0; i < MT; i++) split<XBF>(raw[i][s], x[i]);
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int k = 0; k < PARTS; k++)
+                    x[i][k] = *reinterpret_cast<const bf16x8*>(xs + s * STEP_BYTES + k * PART_BYTES + i * TILE_BYTES);
 #pragma unroll
             for (int t = 0; t < NT; t++) {
-                const bf16x8 w = values8_bf16(d[t][s]);
+                const bf16x8 v = values8_bf16(codes[t][s]);
+                const float scale = w[t].scale(s / STEPS);
 #pragma unroll
                 for (int i = 0; i < MT; i++) {
-                    f32x4 part = {0.f, 0.f, 0.f, 0.f};
+                    if (s % STEPS == 0) part[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int q = Operand<XBF>::PARTS - 1; q >= 0; q--)
-                        part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x[i].p[q]), w, part, 0, 0, 0);
+                    for (int k = PARTS - 1; k >= 0; k--)
+                        part[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[i][k], v, part[i][t], 0, 0, 0);
+                    if (s % STEPS == STEPS - 1) {
 #pragma unroll
-                    for (int r = 0; r < 4; r++) acc[i][t][r] = __builtin_fmaf(part[r], scale[t][s], acc[i][t][r]);
+                        for (int r = 0; r < 4; r++) acc[i][t][r] = __builtin_fmaf(part[i][t][r], scale, acc[i][t][r]);
+                    }
                 }
             }
         }
+    };
+    int turn = 0;
+    for (int base = first - SLICE; base < end; base += SLICE) {  // the first time round there is no slice yet
+        const bool more = base + SLICE < end;
+        if (more) load_x(base + SLICE);
+        if (base >= first) {
+            const int stop = min(turns_all, turn + (1 << log_turns));
+            // a whole slice has a multiple of DEPTH turns
+            for (; turn < stop; turn += DEPTH) {
+#pragma unroll
+                for (int d = 0; d < DEPTH; d++) {
+                    if (turn + d < stop) chunk(w[d], turn + d, base);
+                    load(w[d], turn + d + DEPTH);
+                    asm volatile("" ::: "memory");  // the loads stay here, turns ahead of their use
+                }
+            }
+            __syncthreads();
+        }
+        if (more) {
+            stage_x(base + SLICE);
+            __syncthreads();
+        }
     }
-    // lane (ln, lj) holds column ln, rows 4 lj .. 4 lj + 3 of each 16 x 16 tile
+
+    // lane (ln, lj) holds column ln, rows 4 lj .. 4 lj + 3 of each 16 x 16 tile; the wavefronts of a column add up
+    f32x4* sums = reinterpret_cast<f32x4*>(lds);  // [wavefronts][NT][64]
 #pragma unroll
     for (int i = 0; i < MT; i++) {
         if (i) __syncthreads();
 #pragma unroll
         for (int t = 0; t < NT; t++) sums[(wave * NT + t) * 64 + lane] = acc[i][t];
         __syncthreads();
-        for (int e = threadIdx.x; e < NT * 64; e += blockDim.x) {
-            f32x4 y = sums[e];
-            for (int w = 1; w < waves; w++) {
-                const f32x4 z = sums[w * NT * 64 + e];
+        for (int e = threadIdx.x; e < columns * NT * 64; e += 64 * WAVES) {
+            const int group = e / (NT * 64), rest = e % (NT * 64);
+            f32x4 y = sums[group * kw * NT * 64 + rest];
+            for (int k = 1; k < kw; k++) {
+                const f32x4 z = sums[(group * kw + k) * NT * 64 + rest];
 #pragma unroll
                 for (int r = 0; r < 4; r++) y[r] += z[r];
             }
-            const long n = n0 + (e >> 6) * 16 + (e & 15);
-            const long m = m0 + i * 16 + ((e & 63) >> 4) * 4;
+            const long n = ((long)blockIdx.x * columns + group) * (16 * NT) + (rest >> 6) * 16 + (rest & 15);
+            const int at = ((rest & 63) >> 4) * 4;  // row in the tile
 #pragma unroll
-            for (int r = 0; r < 4; r++)
-                if (n < a.N && m + r < a.M) store_y(a, (m + r) * a.ldy + n, y[r]);
+            for (int r = 0; r < 4; r++) {
+                const long m = m0 + i * R + at + r;
+                if (n >= a.N || at + r >= R || m >= a.M) continue;
+                if (g.partial) g.partial[((long)blockIdx.z * a.M + m) * a.N + n] = y[r];
+                else store_y(a, m * a.ldy + n, y[r]);
+            }
         }
     }
 }
 
-template <int MT, int NT, bool XBF, int GROUP>
-void launch_gemm(const W4Args& a) {
-    const int chunks = (a.K + 127) / 128;
-    int waves = 8;
-    while (waves > 1 && waves / 2 >= chunks) waves /= 2;
-    hipLaunchKernelGGL((gemm_w4_kernel<MT, NT, XBF, GROUP>),
-                       dim3((unsigned)((a.N + 16L * NT - 1) / (16 * NT)), (unsigned)((a.M + 16L * MT - 1) / (16 * MT))),
-                       dim3(64 * waves), waves * NT * 64 * sizeof(f32x4), stream(), a);
+// the parts of a split contraction, added in their order
+__global__ __launch_bounds__(256) void join_w4_kernel(const W4Args a, const float* partial, int parts) {
+    const long id = (long)blockIdx.x * 256 + threadIdx.x, size = (long)a.M * a.N;
+    if (id >= size) return;
+    float y = partial[id];
+    for (int p = 1; p < parts; p++) y += partial[p * size + id];
+    const long m = id / a.N;
+    store_y(a, m * a.ldy + (id - m * a.N), y);
 }
-template <int MT, int NT>
-void launch_gemm(const W4Args& a) {
-    if (a.x_bf16) {
-        if (a.group == 32) launch_gemm<MT, NT, true, 32>(a);
-        else if (a.group == 64) launch_gemm<MT, NT, true, 64>(a);
-        else launch_gemm<MT, NT, true, 128>(a);
-    } else {
-        if (a.group == 32) launch_gemm<MT, NT, false, 32>(a);
-        else if (a.group == 64) launch_gemm<MT, NT, false, 64>(a);
-        else launch_gemm<MT, NT, false, 128>(a);
+
+struct GemmPlan {
+    int r, mt, nt, log_kw, parts, split_chunks;
+};
+
+#ifdef TUNE
+}}
+extern "C" { int tune[8]; }
+namespace nerf { namespace {
+#endif
+
+GemmPlan plan_gemm(int M, int N, int K) {
+    GemmPlan p = {};
+    const int chunks = K / 128 + (K % 128 != 0);
+    p.r = M <= 4 ? 4 : 16;
+    p.mt = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+    p.nt = N >= 8192 ? 2 : 1;
+    const int slice = slice_chunks(p.r, p.mt);
+    const long m_blocks = (M + p.r * p.mt - 1L) / (p.r * p.mt);
+    auto blocks = [&] { return ((long)N + 16 * p.nt * (WAVES >> p.log_kw) - 1) / (16 * p.nt * (WAVES >> p.log_kw)) * m_blocks; };
+    while (blocks() < 128 && (slice >> p.log_kw) > DEPTH && (chunks >> p.log_kw) > 1 && p.log_kw < 3) p.log_kw++;
+    p.parts = (int)std::max(1L, std::min(std::min(16L, chunks / 4L), 256 / blocks()));
+#ifdef TUNE
+    if (tune[0]) p.nt = tune[0];
+    if (tune[1]) p.log_kw = tune[1] - 1;
+    if (tune[2]) p.parts = tune[2];
+    while (p.log_kw && ((slice >> p.log_kw) < DEPTH || (chunks >> p.log_kw) < 1)) p.log_kw--;
+#endif
+    p.split_chunks = (chunks + p.parts - 1) / p.parts;
+    if (p.parts > 1 && p.split_chunks > slice) p.split_chunks = (p.split_chunks + slice - 1) / slice * slice;
+    p.parts = (chunks + p.split_chunks - 1) / p.split_chunks;
+    return p;
+}
+
+template <int R, int MT, int NT, bool XBF, int GROUP>
+hipError_t launch_gemm(const W4Args& a, const GemmPlan& p, float* partial) {
+    constexpr int PARTS = XBF ? 1 : 3;
+    const size_t x_bytes = (size_t)std::min(slice_chunks(R, MT), p.split_chunks) * 4 * (PARTS * MT * R * 64 + 16);
+    const size_t bytes = std::max(x_bytes, (size_t)WAVES * NT * 64 * 16);
+    const long columns = 16L * NT * (WAVES >> p.log_kw);
+    const dim3 grid((unsigned)((a.N + columns - 1) / columns), (unsigned)((a.M + R * MT - 1L) / (R * MT)), (unsigned)p.parts);
+    const GemmShape shape = {p.log_kw, p.split_chunks, p.parts > 1 ? partial : nullptr};
+    hipLaunchKernelGGL((gemm_w4_kernel<R, MT, NT, XBF, GROUP>), grid, dim3(64 * WAVES), bytes, stream(), a, shape);
+    if (p.parts > 1) {
+        const long size = (long)a.M * a.N;
+        hipLaunchKernelGGL(join_w4_kernel, dim3((unsigned)((size + 255) / 256)), dim3(256), 0, stream(), a, partial, p.parts);
     }
+    return hipGetLastError();
+}
+template <int R, int MT, int NT>
+hipError_t launch_gemm(const W4Args& a, const GemmPlan& p, float* partial) {
+    if (a.x_bf16) {
+        if (a.group == 32) return launch_gemm<R, MT, NT, true, 32>(a, p, partial);
+        if (a.group == 64) return launch_gemm<R, MT, NT, true, 64>(a, p, partial);
+        return launch_gemm<R, MT, NT, true, 128>(a, p, partial);
+    }
+    if (a.group == 32) return launch_gemm<R, MT, NT, false, 32>(a, p, partial);
+    if (a.group == 64) return launch_gemm<R, MT, NT, false, 64>(a, p, partial);
+    return launch_gemm<R, MT, NT, false, 128>(a, p, partial);
+}
+template <int R, int MT>
+hipError_t launch_gemm(const W4Args& a, const GemmPlan& p, float* partial) {
+    return p.nt == 1 ? launch_gemm<R, MT, 1>(a, p, partial) : launch_gemm<R, MT, 2>(a, p, partial);
+}
+
+template <int M>
+hipError_t launch_gemv(const W4Args& a) {
+    const int units = a.K / 32 + (a.K % 32 != 0);
+    GemvShape g = {0, 0, GEMV_LOADS, 0};
+    while (g.log_lanes < 6 && (1 << g.log_lanes) < units) g.log_lanes++;
+    while (g.log_kw < 3 && (64 << g.log_kw) < units) g.log_kw++;
+    g.stride = std::max(16, 1 << (g.log_lanes + g.log_kw)) * 16 + 128;
+    // As few rows to a wavefront as leave one workgroup per CU, or two where X takes no LDS: 1 x 16384 x 8192 in bf16
+    // takes 23.1, 16.5, 13.8, 13.0 and 13.9 us with 2, 4, 8, 16 and 32 loads (512 workgroups with 16), in fp32 14.6 us with 32
+    // (256 workgroups) and 15.1 with 16; 1 x 512 x 512 takes 3.1 us with 2 and 5.0 with 8.
+    const long row = (64 >> g.log_lanes) * (WAVES >> g.log_kw);
+    while (g.loads < 32 && g.loads * row < 4096 && a.N / (g.loads * row) >= (a.x_bf16 ? 512 : 256) + 1) g.loads *= 2;
+#ifdef TUNE
+    if (tune[4]) g.loads = tune[4];
+#endif
+    const long block_rows = g.loads * row;
+    const dim3 grid((unsigned)((a.N + block_rows - 1) / block_rows));
+    const size_t bytes = (a.x_bf16 ? 0 : (size_t)M * 8 * g.stride) + (size_t)block_rows * (M << g.log_kw) * sizeof(float);
+    if (a.x_bf16) hipLaunchKernelGGL((gemv_w4_kernel<M, true>), grid, dim3(64 * WAVES), bytes, stream(), a, g);
+    else hipLaunchKernelGGL((gemv_w4_kernel<M, false>), grid, dim3(64 * WAVES), bytes, stream(), a, g);
+    return hipGetLastError();
 }
 
 bool group_ok(int group) { return group == 32 || group == 64 || group == 128; }
@@ -411,8 +776,10 @@ int nerf_dequantize_w4(const unsigned char* d_codes, const unsigned short* d_sca
 }
 
 size_t nerf_gemm_w4_workspace(int M, int N, int K) {
-    (void)M; (void)N; (void)K;
-    return 0;
+    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    if (M <= 2) return 0;
+    const GemmPlan p = plan_gemm(M, N, K);
+    return p.parts > 1 ? (size_t)p.parts * M * N * sizeof(float) : 0;
 }
 
 int nerf_gemm_w4(const void* d_X, int x_type, long ldx, const unsigned char* d_codes, const unsigned short* d_scales,
@@ -431,15 +798,15 @@ int nerf_gemm_w4(const void* d_X, int x_type, long ldx, const unsigned char* d_c
     a.M = M; a.N = N; a.K = K; a.group = group; a.groups = ceil_div(K, group);
     a.x_bf16 = x_type == NERF_TYPE_BF16; a.y_bf16 = y_type == NERF_TYPE_BF16; a.epilogue = epilogue;
     ProfScope prof(K_GEMM_W4, 2.0 * M * N * K);
-    if (M <= 16) {
-        if (N >= 8192) launch_gemm<1, 4>(a);
-        else launch_gemm<1, 1>(a);
-    } else if (M <= 32) {
-        launch_gemm<2, 2>(a);
-    } else {
-        launch_gemm<4, 2>(a);
-    }
-    return hipGetLastError() == hipSuccess ? NERF_OK : NERF_ERR_HIP;
+    const GemmPlan p = plan_gemm(M, N, K);
+    float* partial = (float*)d_workspace;
+    hipError_t rc;
+    if (M == 1) rc = launch_gemv<1>(a);
+    else if (M == 2) rc = launch_gemv<2>(a);
+    else if (p.mt == 4) rc = launch_gemm<16, 4>(a, p, partial);
+    else if (p.mt == 2) rc = launch_gemm<16, 2>(a, p, partial);
+    else rc = p.r == 16 ? launch_gemm<16, 1>(a, p, partial) : launch_gemm<4, 1>(a, p, partial);
+    return rc == hipSuccess ? NERF_OK : NERF_ERR_HIP;
 }
 
 }  // extern "C"

@@ -120,7 +120,10 @@ def check(got, x, w, y_bf16, epilogue):
 SHAPES = [(1, 1, 1), (1, 3, 31), (1, 17, 33), (2, 64, 32), (1, 512, 512), (1, 100, 150), (1, 130, 2049), (1, 64, 16384), (2, 33, 4090),
           (1, 1000, 64), (1, 9, 20000), (3, 16, 128), (4, 15, 127), (5, 48, 129), (8, 130, 512), (15, 31, 100), (16, 512, 512),
           (16, 16, 16384), (17, 65, 257), (24, 300, 1000), (33, 64, 640), (48, 100, 150), (64, 256, 512), (64, 40, 8200), (65, 70, 96),
-          (100, 130, 300), (129, 17, 64), (1, 4099, 96), (2, 5000, 40), (64, 1030, 64)]
+          (100, 130, 300), (129, 17, 64), (1, 4099, 96), (2, 5000, 40), (64, 1030, 64),
+          # long rows in several rounds or slices, and rows of W that end inside a wavefront's share
+          (2, 70, 16384), (1, 5, 40000), (2, 9, 33000), (1, 2000, 1000), (2, 700, 8), (1, 70000, 24), (3, 35, 20000), (20, 40, 5000),
+          (64, 9000, 200)]
 
 
 @pytest.mark.parametrize("group", [32, 64, 128])
