@@ -1,9 +1,14 @@
 // optimizer.hip -- one AdamW step over many tensors, its 8-bit states, and the global gradient norm.
 //
 // No counterpart in the reference, which updates each matrix of its two MLPs on its own
-// (update_weights_mlp, train.c:219-220).  A plan (NerfAdamw) holds a table of the tensors and a table of
-// chunks -- a chunk is a run of elements of one tensor, the work of one workgroup -- so a step over any
-// number of tensors is ONE launch.
+// (update_weights_mlp, train.c:219-220).  A plan (NerfAdamw) holds a table of chunks -- a chunk is a run of up to
+// 4096 elements of one tensor, the work of four workgroups -- so a step over any number of tensors is ONE launch.
+// A chunk's record holds its addresses themselves: one dependent read in front of the data.
+//
+// Everything here waits for memory.  A workgroup takes 1024 elements, four to a thread: all it reads is asked for
+// before the first use, and there are always others to take over while it waits (134 million elements, bf16 gradients
+// and copy, 28 bytes an element: 623 us = 6.0 TB/s; with 2048, 4096 and 8192 elements to a workgroup 658, 671 and
+// 684 us; a loop over the pieces does not overlap them as well as the scheduler does).
 #include "common.hpp"
 #include "../../include/nerf_amd.h"
 
@@ -20,35 +25,47 @@ namespace {
 
 // Elements that share an exponent in the 8-bit states: one wavefront's four consecutive elements per lane.
 constexpr unsigned BLOCK = 256;
-constexpr unsigned NORM_BLOCKS = 1024;  // workgroups, and partial sums, of the norm
+constexpr unsigned NORM_BLOCKS = 512, NORM_WAVES = 16;  // workgroups, and partial sums, of the norm; wavefronts of one
+constexpr unsigned CHUNK = 4096, PIECE = 1024, PIECES = CHUNK / PIECE;  // elements of a record, of a workgroup
 
-// pieces of four elements at any element-aligned address
+// pieces of elements at any element-aligned address
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned short u16x4u __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned short u16x8u __attribute__((ext_vector_type(8), aligned(2)));
 typedef unsigned u32u __attribute__((aligned(1)));
+// Pointers out of the plan's table are to device memory: saying so keeps their loads off the generic path
+#define GLOBAL __attribute__((address_space(1)))
+typedef GLOBAL const f32x4u* LoadF32x4;
+typedef GLOBAL f32x4u* StoreF32x4;
+typedef GLOBAL const u16x4u* LoadU16x4;
+typedef GLOBAL u16x4u* StoreU16x4;
+typedef GLOBAL const u16x8u* LoadU16x8;
+typedef GLOBAL const u32u* LoadU32;
+typedef GLOBAL u32u* StoreU32;
+typedef GLOBAL const float* LoadF32;
+typedef GLOBAL float* StoreF32;
+typedef GLOBAL const unsigned short* LoadU16;
+typedef GLOBAL unsigned short* StoreU16;
+typedef GLOBAL const unsigned char* LoadU8;
+typedef GLOBAL unsigned char* StoreU8;
 
-struct Tensor {
-    float* w;
+struct Chunk {
+    float* w;  // the chunk's first elements
     const void* g;
     void* m;
     void* v;
     unsigned char* m_exp;
     unsigned char* v_exp;
     unsigned short* w_bf16;
-    size_t n;
-    size_t first;  // elements of the tensors before this one
+    size_t first;    // elements of the whole list before it
+    unsigned count;  // elements, at most the plan's chunk
+    unsigned tensor, block;  // place in the list; blocks of the tensor before it
     float lr_scale, weight_decay;
     int g_bf16;
-    unsigned index;
-};
-struct Chunk {
-    unsigned tensor, number;  // elements [number * chunk, (number + 1) * chunk) of the tensor
 };
 
 struct StepArgs {
-    const Tensor* tensors;
     const Chunk* chunks;
-    unsigned chunk;  // elements, a multiple of 1024
     float lr, root_c2t, c1t;      // learning rate, sqrt(1 - beta2^t), 1 - beta1^t
     float grad_div, grad_mul;     // grad_mul: 1 / grad_div where that is exact, else 0
     float beta1, beta2, eps;
@@ -71,44 +88,76 @@ __host__ __device__ __forceinline__ unsigned mix32(unsigned x) {
     return x ^ (x >> 16);
 }
 
-// up to four consecutive elements; `left` of them exist
+// Up to four consecutive elements; `left` of them exist.  STREAM: past the caches, for data that is larger than they are.
+template <bool STREAM>
 __device__ __forceinline__ f32x4u load4(const float* p, unsigned left) {
-    if (left >= 4) return *reinterpret_cast<const f32x4u*>(p);
+    if (left >= 4) return STREAM ? __builtin_nontemporal_load((LoadF32x4)p) : *(LoadF32x4)p;
     f32x4u x = {0.f, 0.f, 0.f, 0.f};
-    for (unsigned k = 0; k < left; k++) x[k] = p[k];
+#pragma unroll
+    for (unsigned k = 0; k < 3; k++)
+        if (k < left) x[k] = ((LoadF32)p)[k];
     return x;
 }
+template <bool STREAM>
 __device__ __forceinline__ f32x4u load4(const unsigned short* p, unsigned left) {
     u16x4u b = {0, 0, 0, 0};
-    if (left >= 4) b = *reinterpret_cast<const u16x4u*>(p);
+    if (left >= 4) b = STREAM ? __builtin_nontemporal_load((LoadU16x4)p) : *(LoadU16x4)p;
     else
-        for (unsigned k = 0; k < left; k++) b[k] = p[k];
+#pragma unroll
+        for (unsigned k = 0; k < 3; k++)
+            if (k < left) b[k] = ((LoadU16)p)[k];
     f32x4u x;
+#pragma unroll
     for (int k = 0; k < 4; k++) x[k] = bf16_to_f32(b[k]);
     return x;
 }
+template <bool STREAM>
 __device__ __forceinline__ unsigned load4(const unsigned char* p, unsigned left) {
-    if (left >= 4) return *reinterpret_cast<const u32u*>(p);
+    if (left >= 4) return STREAM ? __builtin_nontemporal_load((LoadU32)p) : *(LoadU32)p;
     unsigned x = 0;
-    for (unsigned k = 0; k < left; k++) x |= (unsigned)p[k] << (8 * k);
+#pragma unroll
+    for (unsigned k = 0; k < 3; k++)
+        if (k < left) x |= (unsigned)((LoadU8)p)[k] << (8 * k);
     return x;
 }
+template <bool STREAM>
 __device__ __forceinline__ void store4(float* p, f32x4u x, unsigned left) {
-    if (left >= 4) *reinterpret_cast<f32x4u*>(p) = x;
-    else
-        for (unsigned k = 0; k < left; k++) p[k] = x[k];
+    if (left < 4) {
+#pragma unroll
+        for (unsigned k = 0; k < 3; k++)
+            if (k < left) ((StoreF32)p)[k] = x[k];
+    } else if (STREAM) {
+        __builtin_nontemporal_store(x, (StoreF32x4)p);
+    } else {
+        *(StoreF32x4)p = x;
+    }
 }
+template <bool STREAM>
 __device__ __forceinline__ void store4_bf16(unsigned short* p, f32x4u x, unsigned left) {
     u16x4u b;
+#pragma unroll
     for (int k = 0; k < 4; k++) b[k] = f32_to_bf16(x[k]);
-    if (left >= 4) *reinterpret_cast<u16x4u*>(p) = b;
-    else
-        for (unsigned k = 0; k < left; k++) p[k] = b[k];
+    if (left < 4) {
+#pragma unroll
+        for (unsigned k = 0; k < 3; k++)
+            if (k < left) ((StoreU16)p)[k] = b[k];
+    } else if (STREAM) {
+        __builtin_nontemporal_store(b, (StoreU16x4)p);
+    } else {
+        *(StoreU16x4)p = b;
+    }
 }
+template <bool STREAM>
 __device__ __forceinline__ void store4(unsigned char* p, unsigned x, unsigned left) {
-    if (left >= 4) *reinterpret_cast<u32u*>(p) = x;
-    else
-        for (unsigned k = 0; k < left; k++) p[k] = (unsigned char)(x >> (8 * k));
+    if (left < 4) {
+#pragma unroll
+        for (unsigned k = 0; k < 3; k++)
+            if (k < left) ((StoreU8)p)[k] = (unsigned char)(x >> (8 * k));
+    } else if (STREAM) {
+        __builtin_nontemporal_store(x, (StoreU32)p);
+    } else {
+        *(StoreU32)p = x;
+    }
 }
 
 // What an element's gradient is multiplied by beyond the divisor; false: the step is left out (the norm is not
@@ -128,36 +177,55 @@ __device__ __forceinline__ float gradient(const StepArgs& a, float g, float fact
     return __fmul_rn(x, factor);
 }
 
+template <bool STREAM>
+__device__ __forceinline__ f32x4u load_g(const Chunk& c, unsigned i, unsigned left) {
+    return c.g_bf16 ? load4<STREAM>((const unsigned short*)c.g + i, left) : load4<STREAM>((const float*)c.g + i, left);
+}
+
+// The chunk of a workgroup, and the step's factors for its tensor; false: nothing to do
+struct Piece {
+    Chunk c;
+    float factor, alpha, decay;
+
+    __device__ __forceinline__ bool of(const StepArgs& a) {
+        c = a.chunks[blockIdx.x / PIECES];
+        if (!clip_factor(a, factor) || blockIdx.x % PIECES * PIECE >= c.count) return false;
+        const float lr = __fmul_rn(a.lr, c.lr_scale);
+        alpha = __fdiv_rn(__fmul_rn(lr, a.root_c2t), a.c1t);
+        decay = __fsub_rn(1.0f, __fmul_rn(lr, c.weight_decay));
+        return true;
+    }
+};
+
 // ---- 32-bit states --------------------------------------------------------------------------------------
 // The operations of adamw_element (mlp.hip) in the same order: the same bits as nerf_trainer_update.
-__global__ __launch_bounds__(256) void adamw32_kernel(const StepArgs a) {
-    const Chunk c = a.chunks[blockIdx.x];
-    const Tensor t = a.tensors[c.tensor];
-    float factor;
-    if (!clip_factor(a, factor)) return;
-    const float lr = __fmul_rn(a.lr, t.lr_scale);
-    const float alpha = __fdiv_rn(__fmul_rn(lr, a.root_c2t), a.c1t);
-    const float decay = __fsub_rn(1.0f, __fmul_rn(lr, t.weight_decay));
+template <bool STREAM>
+__device__ __forceinline__ void adamw32_four(const StepArgs& a, const Piece& p, unsigned i, unsigned left) {
+    const Chunk& c = p.c;
     const float c1 = __fsub_rn(1.0f, a.beta1), c2 = __fsub_rn(1.0f, a.beta2);
-    const size_t begin = (size_t)c.number * a.chunk;
-    const size_t end = min(t.n, begin + a.chunk);
-    for (size_t i = begin + threadIdx.x * 4; i < end; i += 1024) {
-        const unsigned left = (unsigned)min((size_t)4, end - i);
-        f32x4u w = load4(t.w + i, left), m = load4((float*)t.m + i, left), v = load4((float*)t.v + i, left);
-        const f32x4u g = t.g_bf16 ? load4((const unsigned short*)t.g + i, left) : load4((const float*)t.g + i, left);
+    f32x4u w = load4<STREAM>(c.w + i, left), m = load4<STREAM>((float*)c.m + i, left), v = load4<STREAM>((float*)c.v + i, left);
+    const f32x4u g = load_g<STREAM>(c, i, left);
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const float gi = gradient(a, g[k], factor);
-            m[k] = __fadd_rn(__fmul_rn(a.beta1, m[k]), __fmul_rn(c1, gi));
-            v[k] = __fadd_rn(__fmul_rn(a.beta2, v[k]), __fmul_rn(__fmul_rn(c2, gi), gi));
-            const float up = __fdiv_rn(__fmul_rn(alpha, m[k]), __fadd_rn(sqrtf(v[k]), a.eps));
-            w[k] = __fsub_rn(__fmul_rn(w[k], decay), up);
-        }
-        store4((float*)t.m + i, m, left);
-        store4((float*)t.v + i, v, left);
-        store4(t.w + i, w, left);
-        if (t.w_bf16) store4_bf16(t.w_bf16 + i, w, left);
+    for (int k = 0; k < 4; k++) {
+        const float gi = gradient(a, g[k], p.factor);
+        m[k] = __fadd_rn(__fmul_rn(a.beta1, m[k]), __fmul_rn(c1, gi));
+        v[k] = __fadd_rn(__fmul_rn(a.beta2, v[k]), __fmul_rn(__fmul_rn(c2, gi), gi));
+        const float up = __fdiv_rn(__fmul_rn(p.alpha, m[k]), __fadd_rn(sqrtf(v[k]), a.eps));
+        w[k] = __fsub_rn(__fmul_rn(w[k], p.decay), up);
     }
+    store4<STREAM>((float*)c.m + i, m, left);
+    store4<STREAM>((float*)c.v + i, v, left);
+    store4<STREAM>(c.w + i, w, left);
+    if (c.w_bf16) store4_bf16<STREAM>(c.w_bf16 + i, w, left);
+}
+
+template <bool STREAM>
+__global__ __launch_bounds__(256) void adamw32_kernel(const StepArgs a) {
+    Piece p;
+    if (!p.of(a)) return;
+    const unsigned begin = blockIdx.x % PIECES * PIECE, i = begin + threadIdx.x * 4;
+    if (begin + PIECE <= p.c.count) adamw32_four<STREAM>(a, p, i, 4);
+    else if (i < p.c.count) adamw32_four<STREAM>(a, p, i, min(4u, p.c.count - i));
 }
 
 // ---- 8-bit states ---------------------------------------------------------------------------------------
@@ -196,95 +264,84 @@ __device__ __forceinline__ int block_exponent(unsigned top, int low) {
     return min(max(e, 16), 254);
 }
 
-__global__ __launch_bounds__(256) void adamw8_kernel(const StepArgs a, const int stochastic) {
-    const Chunk c = a.chunks[blockIdx.x];
-    const Tensor t = a.tensors[c.tensor];
-    float factor;
-    if (!clip_factor(a, factor)) return;
-    const float lr = __fmul_rn(a.lr, t.lr_scale);
-    const float alpha = __fdiv_rn(__fmul_rn(lr, a.root_c2t), a.c1t);
-    const float decay = __fsub_rn(1.0f, __fmul_rn(lr, t.weight_decay));
+// A wavefront takes a whole block, four consecutive elements to a lane; every lane stays, those past the end with nothing
+// `left`.
+template <bool STOCHASTIC, bool STREAM>
+__device__ __forceinline__ void adamw8_block(const StepArgs& a, const Piece& p, unsigned i, unsigned left) {
+    const Chunk& c = p.c;
     const float c1 = __fsub_rn(1.0f, a.beta1), c2 = __fsub_rn(1.0f, a.beta2);
-    const unsigned tensor_key = mix32(a.key + t.index * 0x9E3779B9u);
-    unsigned char *mc = (unsigned char*)t.m, *vc = (unsigned char*)t.v;
-    const size_t begin = (size_t)c.number * a.chunk;
-    const size_t end = min(t.n, begin + a.chunk);
     const int lane = threadIdx.x & 63;
-    // a wavefront takes a whole block: every lane stays in the loop, those past the end with nothing left
-    for (size_t b0 = begin + (threadIdx.x >> 6) * BLOCK; b0 < end; b0 += 1024) {
-        const size_t block = b0 / BLOCK;
-        const size_t i = b0 + lane * 4;
-        const unsigned left = i < end ? (unsigned)min((size_t)4, end - i) : 0;
-        f32x4u w = {0.f, 0.f, 0.f, 0.f}, g = {0.f, 0.f, 0.f, 0.f};
-        unsigned m_old = 0, v_old = 0;
-        if (left) {
-            w = load4(t.w + i, left);
-            m_old = load4(mc + i, left);
-            v_old = load4(vc + i, left);
-            g = t.g_bf16 ? load4((const unsigned short*)t.g + i, left) : load4((const float*)t.g + i, left);
-        }
-        const int m_e = t.m_exp[block], v_e = t.v_exp[block];
-        float m[4], r[4];
-        unsigned m_top = 0, r_top = 0;
+    const unsigned block = __builtin_amdgcn_readfirstlane(i / BLOCK);
+    unsigned char *mc = (unsigned char*)c.m + i, *vc = (unsigned char*)c.v + i;
+    f32x4u w = load4<STREAM>(c.w + i, left);
+    const f32x4u g = load_g<STREAM>(c, i, left);
+    const unsigned m_old = load4<STREAM>(mc, left), v_old = load4<STREAM>(vc, left);
+    const int m_e = ((LoadU8)c.m_exp)[block], v_e = ((LoadU8)c.v_exp)[block];
+    float m[4], r[4];
+    unsigned m_top = 0, r_top = 0;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const unsigned mb = (m_old >> (8 * k)) & 255, vb = (v_old >> (8 * k)) & 255;
-            const float m0 = decode(mb & 127, 20, m_e);
-            const float r0 = decode(vb, 19, v_e);
-            const float gi = gradient(a, g[k], factor);
-            m[k] = __fadd_rn(__fmul_rn(a.beta1, mb & 128 ? -m0 : m0), __fmul_rn(c1, gi));
-            r[k] = sqrtf(__fadd_rn(__fmul_rn(a.beta2, __fmul_rn(r0, r0)), __fmul_rn(__fmul_rn(c2, gi), gi)));
-            const float up = __fdiv_rn(__fmul_rn(alpha, m[k]), __fadd_rn(r[k], a.eps));
-            w[k] = __fsub_rn(__fmul_rn(w[k], decay), up);
-            // a state that is not finite is held as zero and leaves the block's exponent alone
-            if (!(fabsf(m[k]) < INFINITY)) m[k] = 0.0f;
-            if (!(r[k] < INFINITY)) r[k] = 0.0f;
-            m_top = max(m_top, __builtin_bit_cast(unsigned, fabsf(m[k])));
-            r_top = max(r_top, __builtin_bit_cast(unsigned, r[k]));
-        }
-        const int m_new = block_exponent(wave_max(m_top), 20), v_new = block_exponent(wave_max(r_top), 19);
-        const unsigned block_key = mix32(tensor_key + (unsigned)block * 0x85EBCA6Bu);
-        unsigned m_codes = 0, v_codes = 0;
+    for (int k = 0; k < 4; k++) {
+        const unsigned mb = (m_old >> (8 * k)) & 255, vb = (v_old >> (8 * k)) & 255;
+        const float m0 = decode(mb & 127, 20, m_e);
+        const float r0 = decode(vb, 19, v_e);
+        const float gi = gradient(a, g[k], p.factor);
+        m[k] = __fadd_rn(__fmul_rn(a.beta1, mb & 128 ? -m0 : m0), __fmul_rn(c1, gi));
+        r[k] = sqrtf(__fadd_rn(__fmul_rn(a.beta2, __fmul_rn(r0, r0)), __fmul_rn(__fmul_rn(c2, gi), gi)));
+        const float up = __fdiv_rn(__fmul_rn(p.alpha, m[k]), __fadd_rn(r[k], a.eps));
+        w[k] = __fsub_rn(__fmul_rn(w[k], p.decay), up);
+        // a state that is not finite is held as zero and leaves the block's exponent alone
+        if (!(fabsf(m[k]) < INFINITY)) m[k] = 0.0f;
+        if (!(r[k] < INFINITY)) r[k] = 0.0f;
+        m_top = max(m_top, __builtin_bit_cast(unsigned, fabsf(m[k])));
+        r_top = max(r_top, __builtin_bit_cast(unsigned, r[k]));
+    }
+    if (left) store4<STREAM>(c.w + i, w, left);
+    if (left && c.w_bf16) store4_bf16<STREAM>(c.w_bf16 + i, w, left);
+    const int m_new = block_exponent(wave_max(m_top), 20), v_new = block_exponent(wave_max(r_top), 19);
+    const unsigned block_key = mix32(mix32(a.key + c.tensor * 0x9E3779B9u) + (c.block + block) * 0x85EBCA6Bu);
+    unsigned m_codes = 0, v_codes = 0;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            unsigned m_noise = 1u << 19, r_noise = 1u << 18;  // half a step: to nearest
-            if (stochastic) {
-                const unsigned h = mix32(block_key ^ (unsigned)(lane * 4 + k));
-                m_noise = (h & 0xFFFF) << 4;
-                r_noise = (h >> 16) << 3;
-            }
-            unsigned mq = min(encode(fabsf(m[k]), 20, m_new, m_noise), 127u);
-            if (m[k] < 0.0f && mq) mq |= 128;
-            unsigned rq = min(encode(r[k], 19, v_new, r_noise), 255u);
-            // a second moment that is not zero does not become zero: the update divides by its root
-            if (rq == 0 && r[k] > 0.0f) rq = 1;
-            m_codes |= mq << (8 * k);
-            v_codes |= rq << (8 * k);
+    for (int k = 0; k < 4; k++) {
+        unsigned m_noise = 1u << 19, r_noise = 1u << 18;  // half a step: to nearest
+        if (STOCHASTIC) {
+            const unsigned h = mix32(block_key ^ (unsigned)(lane * 4 + k));
+            m_noise = (h & 0xFFFF) << 4;
+            r_noise = (h >> 16) << 3;
         }
-        if (left) {
-            store4(t.w + i, w, left);
-            store4(mc + i, m_codes, left);
-            store4(vc + i, v_codes, left);
-            if (t.w_bf16) store4_bf16(t.w_bf16 + i, w, left);
-        }
-        if (lane == 0) {
-            t.m_exp[block] = (unsigned char)m_new;
-            t.v_exp[block] = (unsigned char)v_new;
-        }
+        unsigned mq = min(encode(fabsf(m[k]), 20, m_new, m_noise), 127u);
+        if (m[k] < 0.0f && mq) mq |= 128;
+        unsigned rq = min(encode(r[k], 19, v_new, r_noise), 255u);
+        // a second moment that is not zero does not become zero: the update divides by its root
+        if (rq == 0 && r[k] > 0.0f) rq = 1;
+        m_codes |= mq << (8 * k);
+        v_codes |= rq << (8 * k);
+    }
+    if (left) {
+        store4<STREAM>(mc, m_codes, left);
+        store4<STREAM>(vc, v_codes, left);
+    }
+    if (lane == 0) {
+        ((StoreU8)c.m_exp)[block] = (unsigned char)m_new;
+        ((StoreU8)c.v_exp)[block] = (unsigned char)v_new;
     }
 }
 
+template <bool STOCHASTIC, bool STREAM>
+__global__ __launch_bounds__(256) void adamw8_kernel(const StepArgs a) {
+    Piece p;
+    if (!p.of(a)) return;
+    const unsigned begin = blockIdx.x % PIECES * PIECE, i = begin + threadIdx.x * 4;
+    if (begin + PIECE <= p.c.count) adamw8_block<STOCHASTIC, STREAM>(a, p, i, 4);
+    else if (i / BLOCK * BLOCK < p.c.count) adamw8_block<STOCHASTIC, STREAM>(a, p, i, i < p.c.count ? min(4u, p.c.count - i) : 0);
+}
+
 // the values that 8-bit states stand for, as bf16 (every one is exact: at most 5 significant bits)
-__global__ __launch_bounds__(256) void read_states_kernel(const Tensor* tensors, const Chunk* chunks, unsigned chunk,
-                                                          unsigned short* m_out, unsigned short* r_out) {
+template <bool STREAM>
+__global__ __launch_bounds__(256) void read_states_kernel(const Chunk* chunks, unsigned short* m_out, unsigned short* r_out) {
     const Chunk c = chunks[blockIdx.x];
-    const Tensor t = tensors[c.tensor];
-    const size_t begin = (size_t)c.number * chunk;
-    const size_t end = min(t.n, begin + chunk);
-    for (size_t i = begin + threadIdx.x * 4; i < end; i += 1024) {
-        const unsigned left = (unsigned)min((size_t)4, end - i);
-        const unsigned mc = load4((const unsigned char*)t.m + i, left), vc = load4((const unsigned char*)t.v + i, left);
-        const int m_e = t.m_exp[i / BLOCK], v_e = t.v_exp[i / BLOCK];
+    auto four = [&](unsigned i, unsigned left) {
+        const unsigned mc = load4<STREAM>((const unsigned char*)c.m + i, left), vc = load4<STREAM>((const unsigned char*)c.v + i, left);
+        const int m_e = ((LoadU8)c.m_exp)[i / BLOCK], v_e = ((LoadU8)c.v_exp)[i / BLOCK];
         f32x4u m, r;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
@@ -293,70 +350,122 @@ __global__ __launch_bounds__(256) void read_states_kernel(const Tensor* tensors,
             m[k] = mb & 128 ? -x : x;
             r[k] = decode(vb, 19, v_e);
         }
-        if (m_out) store4_bf16(m_out + t.first + i, m, left);
-        if (r_out) store4_bf16(r_out + t.first + i, r, left);
-    }
+        if (m_out) store4_bf16<STREAM>(m_out + c.first + i, m, left);
+        if (r_out) store4_bf16<STREAM>(r_out + c.first + i, r, left);
+    };
+    const unsigned whole = c.count & ~1023u;
+    unsigned i = threadIdx.x * 4;
+    for (; i < whole; i += 1024) four(i, 4);
+    if (i < c.count) four(i, min(4u, c.count - i));
 }
 
 // ---- global norm ----------------------------------------------------------------------------------------
 // Squares are added in 64 bits, so neither the range of the squares nor the length of the sum costs anything
-// (the kernel waits for memory).  Each workgroup walks the chunks at a fixed stride and leaves one partial sum;
+// (the kernel waits for memory).  Each wavefront walks the pieces at a fixed stride, each workgroup leaves one partial sum;
 // the workgroup that finishes last adds the partial sums in their order: the same bits on every call.
 __device__ __forceinline__ double block_sum(double x, double* shared) {
 #pragma unroll
     for (int d = 32; d >= 1; d >>= 1) x += __shfl_xor(x, d, 64);
     if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = x;
     __syncthreads();
-    x = shared[0] + shared[1] + shared[2] + shared[3];
+    x = 0.0;
+#pragma unroll
+    for (int w = 0; w < NORM_WAVES; w++) x += shared[w];
     __syncthreads();
     return x;
 }
 
-__global__ __launch_bounds__(256) void grad_norm_kernel(const Tensor* tensors, const Chunk* chunks, unsigned count,
-                                                        unsigned chunk, double* partial, unsigned* ticket,
+// a wavefront's part of the sum of the squares of a chunk's elements from `begin` on, PIECE of them or to the end
+__device__ __forceinline__ double squares(const Chunk& c, unsigned begin) {
+    double sum[4] = {0.0, 0.0, 0.0, 0.0};
+    const unsigned lane = threadIdx.x & 63;
+    auto add = [&](f32x4u g) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) sum[k] += (double)g[k] * (double)g[k];
+    };
+    if (begin + PIECE > c.count) {
+        for (unsigned i = begin + lane * 4; i < c.count; i += 256) add(load_g<false>(c, i, min(4u, c.count - i)));
+    } else if (c.g_bf16) {  // 16 bytes to a lane
+        u16x8u g[2];
+#pragma unroll
+        for (int u = 0; u < 2; u++) g[u] = *(LoadU16x8)((const unsigned short*)c.g + begin + lane * 8 + u * 512);
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            add(f32x4u{bf16_to_f32(g[u][0]), bf16_to_f32(g[u][1]), bf16_to_f32(g[u][2]), bf16_to_f32(g[u][3])});
+            add(f32x4u{bf16_to_f32(g[u][4]), bf16_to_f32(g[u][5]), bf16_to_f32(g[u][6]), bf16_to_f32(g[u][7])});
+        }
+    } else {
+        f32x4u g[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) g[u] = load4<false>((const float*)c.g + begin + lane * 4 + u * 256, 4);
+#pragma unroll
+        for (int u = 0; u < 4; u++) add(g[u]);
+    }
+    return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+
+__global__ __launch_bounds__(64 * NORM_WAVES) void grad_norm_kernel(const Chunk* chunks, unsigned count, unsigned long long* partial, unsigned* ticket,
                                                         float grad_div, float* norm) {
-    __shared__ double shared[4];
+    __shared__ double shared[NORM_WAVES];
     __shared__ bool last;
     double sum = 0.0;
-    for (unsigned b = blockIdx.x; b < count; b += gridDim.x) {
-        const Chunk c = chunks[b];
-        const Tensor t = tensors[c.tensor];
-        const size_t begin = (size_t)c.number * chunk;
-        const size_t end = min(t.n, begin + chunk);
-        for (size_t i = begin + threadIdx.x * 4; i < end; i += 1024) {
-            const unsigned left = (unsigned)min((size_t)4, end - i);
-            const f32x4u g = t.g_bf16 ? load4((const unsigned short*)t.g + i, left) : load4((const float*)t.g + i, left);
-#pragma unroll
-            for (int k = 0; k < 4; k++) sum += (double)g[k] * (double)g[k];
-        }
+    for (unsigned b = blockIdx.x * NORM_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); b < count; b += gridDim.x * NORM_WAVES) {
+        const Chunk c = chunks[b / PIECES];
+        if (b % PIECES * PIECE < c.count) sum += squares(c, b % PIECES * PIECE);
     }
     sum = block_sum(sum, shared);
     if (threadIdx.x == 0) {
-        partial[blockIdx.x] = sum;
-        __threadfence();
-        last = atomicInc(ticket, gridDim.x - 1) == gridDim.x - 1;  // wraps to 0 for the next call
+        // The partial sum goes out, and comes in below, by atomic operations of the whole GPU, and the ticket is drawn
+        // when the exchange has answered (its answer is part of the limit, as zero): all that has to be seen is
+        // at the point where those meet, and no cache has to be written back.
+        const unsigned long long before = __hip_atomic_exchange(partial + blockIdx.x, __builtin_bit_cast(unsigned long long, sum),
+                                                                __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        unsigned none = (unsigned)before;
+        asm volatile("v_and_b32 %0, 0, %0" : "+v"(none));
+        last = atomicInc(ticket, gridDim.x - 1 + none) == gridDim.x - 1;  // the last one takes it back to 0 for the next call
     }
     __syncthreads();
     if (!last) return;
-    __threadfence();
     sum = 0.0;
-    for (unsigned b = threadIdx.x; b < gridDim.x; b += 256) sum += partial[b];
+    for (unsigned b = threadIdx.x; b < gridDim.x; b += 64 * NORM_WAVES)
+        sum += __builtin_bit_cast(double, __hip_atomic_load(partial + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
     sum = block_sum(sum, shared);
     if (threadIdx.x == 0) *norm = (float)(sqrt(sum) / (double)grad_div);
 }
 
 bool finite_not_negative(float x) { return x >= 0.0f && x < INFINITY; }
 
-// Whether `p` may be handed to a kernel on `device`: not pageable host memory, not another GPU's
-bool on_device(const void* p, int device) {
-    hipPointerAttribute_t at;
-    if (hipPointerGetAttributes(&at, p) != hipSuccess) {
-        (void)hipGetLastError();
-        return false;
+// Whether a buffer may be handed to a kernel on a device: inside one allocation, and not pageable host memory or
+// another GPU's.  Tensors mostly come out of a few allocations: the last one found is kept.
+class DevicePointers {
+public:
+    explicit DevicePointers(int device) : device_(device) {}
+    bool holds(const void* p, size_t bytes) {
+        const uintptr_t at = (uintptr_t)p;
+        if (at >= begin_ && at - begin_ < size_) return bytes <= size_ - (at - begin_);
+        hipPointerAttribute_t info;
+        if (hipPointerGetAttributes(&info, p) != hipSuccess) {
+            (void)hipGetLastError();
+            return false;
+        }
+        if (info.type == hipMemoryTypeDevice ? info.device != device_ : info.type != hipMemoryTypeHost && info.type != hipMemoryTypeManaged)
+            return false;
+        hipDeviceptr_t base = nullptr;
+        size_t size = 0;
+        if (hipMemGetAddressRange(&base, &size, (hipDeviceptr_t)p) != hipSuccess) {
+            (void)hipGetLastError();
+            return true;  // known to the runtime, but not as one allocation
+        }
+        begin_ = (uintptr_t)base;
+        size_ = size;
+        return at >= begin_ && at - begin_ < size_ && bytes <= size_ - (at - begin_);
     }
-    if (at.type == hipMemoryTypeDevice) return at.device == device;
-    return at.type == hipMemoryTypeHost || at.type == hipMemoryTypeManaged;
-}
+
+private:
+    int device_;
+    uintptr_t begin_ = 1;
+    size_t size_ = 0;
+};
 
 struct Range {
     uintptr_t begin, end;
@@ -405,16 +514,20 @@ int check_tensors(const NerfAdamwTensor* tensors, int count, int state_bits) {
 
 using namespace nerf;
 
+// Bytes of a step beyond which it streams past the caches (256 MB on the memory side).  Three lists in turn, each with
+// and without: 4 million elements in 32 bits (112 MB) 19.8 and 18.1 us, 8 million (224 MB) 37.7 and 43.3 us, 134 million with
+// bf16 gradients and copy (3.8 GB) 623 and 739 us.
+constexpr double STREAM_BYTES = 160e6;
+
 struct NerfAdamw {
     int device, state_bits;
     float beta1, beta2, eps;
-    unsigned chunk, chunks;
-    size_t elements;
+    unsigned chunks;
     double bytes, grad_bytes;  // of one step, of one norm
-    Tensor* d_tensors;
-    Chunk* d_chunks;
-    double* d_partial;
+    void* memory;              // one allocation: partial sums, ticket, chunks
+    unsigned long long* d_partial;
     unsigned* d_ticket;
+    Chunk* d_chunks;
 };
 
 extern "C" {
@@ -422,43 +535,59 @@ extern "C" {
 size_t nerf_adamw_state_blocks(size_t n) { return n / BLOCK + (n % BLOCK != 0); }
 
 static int build_plan(const NerfAdamwTensor* tensors, int count, int state_bits, NerfAdamw* plan) {
-    std::vector<Tensor> table((size_t)count);
-    std::vector<Chunk> chunks;
-    size_t elements = 0;
-    for (int k = 0; k < count; k++) elements += tensors[k].n;
-    plan->elements = elements;
-    // Up to a million elements a chunk is one piece per thread, so that the few workgroups there are spread over
-    // the chip; beyond that, four
-    plan->chunk = elements <= (1u << 20) ? 1024 : 4096;
+    size_t pieces = 0;
+    for (int k = 0; k < count; k++) {
+        pieces += tensors[k].n / CHUNK + (tensors[k].n % CHUNK != 0);
+        if (pieces > 0xffffffu / PIECES) return NERF_ERR_ARG;  // a launch has fewer than 2^32 threads
+    }
+    constexpr size_t HEAD = NORM_BLOCKS * sizeof(unsigned long long) + 256;
+    std::vector<char> image(HEAD + pieces * sizeof(Chunk));
+    Chunk* table = reinterpret_cast<Chunk*>(image.data() + HEAD);
+    DevicePointers known(plan->device);
     size_t first = 0;
     for (int k = 0; k < count; k++) {
         const NerfAdamwTensor& s = tensors[k];
-        if (s.n) {
-            const void* all[] = {s.g, s.w, s.m, s.v, s.m_exp, s.v_exp, s.w_bf16};
-            const int used = state_bits == 0 ? 1 : state_bits == 32 ? 4 : 6;
-            for (int p = 0; p < 7; p++)
-                if ((p < used || (p == 6 && state_bits && s.w_bf16)) && !on_device(all[p], plan->device)) return NERF_ERR_ARG;
-        }
-        table[k] = Tensor{s.w, s.g, s.m, s.v, s.m_exp, s.v_exp, s.w_bf16, s.n, first, s.lr_scale, s.weight_decay,
-                          s.grad_type == NERF_TYPE_BF16, (unsigned)k};
-        const double g_item = s.grad_type == NERF_TYPE_BF16 ? 2.0 : 4.0;
+        if (s.n == 0) continue;
+        const bool bf = s.grad_type == NERF_TYPE_BF16;
+        const size_t state = state_bits == 8 ? 1 : 4, blocks = nerf_adamw_state_blocks(s.n);
+        bool ok = known.holds(s.g, s.n * (bf ? 2 : 4));
+        if (state_bits) ok = ok && known.holds(s.w, s.n * 4) && known.holds(s.m, s.n * state) && known.holds(s.v, s.n * state);
+        if (state_bits == 8) ok = ok && known.holds(s.m_exp, blocks) && known.holds(s.v_exp, blocks);
+        if (state_bits && s.w_bf16) ok = ok && known.holds(s.w_bf16, s.n * 2);
+        if (!ok) return NERF_ERR_ARG;
+        const double g_item = bf ? 2.0 : 4.0;
         plan->grad_bytes += (double)s.n * g_item;
-        plan->bytes += (double)s.n * (8.0 + g_item + (state_bits == 8 ? 4.0 : 16.0) + (s.w_bf16 ? 2.0 : 0.0));
+        plan->bytes += (double)s.n * (8.0 + g_item + 4.0 * (double)state + (s.w_bf16 ? 2.0 : 0.0));
+        for (size_t at = 0; at < s.n; at += CHUNK) {
+            Chunk c = {};
+            c.g = (const char*)s.g + at * (bf ? 2 : 4);
+            c.g_bf16 = bf;
+            c.count = (unsigned)std::min((size_t)CHUNK, s.n - at);
+            if (state_bits) {
+                c.w = s.w + at;
+                c.m = (char*)s.m + at * state;
+                c.v = (char*)s.v + at * state;
+                c.w_bf16 = s.w_bf16 ? s.w_bf16 + at : nullptr;
+                c.lr_scale = s.lr_scale;
+                c.weight_decay = s.weight_decay;
+            }
+            if (state_bits == 8) {
+                c.m_exp = s.m_exp + at / BLOCK;
+                c.v_exp = s.v_exp + at / BLOCK;
+            }
+            c.first = first + at;
+            c.tensor = (unsigned)k;
+            c.block = (unsigned)(at / BLOCK);
+            *table++ = c;
+        }
         first += s.n;
-        const size_t pieces = s.n / plan->chunk + (s.n % plan->chunk != 0);
-        if (chunks.size() + pieces > 0xffffffu) return NERF_ERR_ARG;  // a launch has fewer than 2^32 threads
-        for (size_t p = 0; p < pieces; p++) chunks.push_back(Chunk{(unsigned)k, (unsigned)p});
     }
-    plan->chunks = (unsigned)chunks.size();
-    if (hipMalloc((void**)&plan->d_tensors, table.size() * sizeof(Tensor)) != hipSuccess) return NERF_ERR_HIP;
-    if (hipMalloc((void**)&plan->d_chunks, (chunks.size() + 1) * sizeof(Chunk)) != hipSuccess) return NERF_ERR_HIP;
-    if (hipMalloc((void**)&plan->d_partial, NORM_BLOCKS * sizeof(double)) != hipSuccess) return NERF_ERR_HIP;
-    if (hipMalloc((void**)&plan->d_ticket, sizeof(unsigned)) != hipSuccess) return NERF_ERR_HIP;
-    const unsigned zero = 0;
-    if (hipMemcpyAsync(plan->d_tensors, table.data(), table.size() * sizeof(Tensor), hipMemcpyHostToDevice, stream()) != hipSuccess ||
-        (plan->chunks && hipMemcpyAsync(plan->d_chunks, chunks.data(), chunks.size() * sizeof(Chunk), hipMemcpyHostToDevice,
-                                        stream()) != hipSuccess) ||
-        hipMemcpyAsync(plan->d_ticket, &zero, sizeof(zero), hipMemcpyHostToDevice, stream()) != hipSuccess ||
+    plan->chunks = (unsigned)pieces;
+    if (hipMalloc(&plan->memory, image.size()) != hipSuccess) return NERF_ERR_HIP;
+    plan->d_partial = (unsigned long long*)plan->memory;
+    plan->d_ticket = (unsigned*)((char*)plan->memory + NORM_BLOCKS * sizeof(unsigned long long));
+    plan->d_chunks = (Chunk*)((char*)plan->memory + HEAD);
+    if (hipMemcpyAsync(plan->memory, image.data(), image.size(), hipMemcpyHostToDevice, stream()) != hipSuccess ||
         hipStreamSynchronize(stream()) != hipSuccess)
         return NERF_ERR_HIP;
     return NERF_OK;
@@ -495,10 +624,7 @@ int nerf_adamw_create(const NerfAdamwTensor* tensors, int count, int state_bits,
 
 void nerf_adamw_destroy(NerfAdamw* plan) {
     if (!plan) return;
-    (void)hipFree(plan->d_tensors);
-    (void)hipFree(plan->d_chunks);
-    (void)hipFree(plan->d_partial);
-    (void)hipFree(plan->d_ticket);
+    (void)hipFree(plan->memory);
     delete plan;
 }
 
@@ -519,9 +645,7 @@ int nerf_adamw_step(NerfAdamw* plan, int step, float learning_rate, float grad_d
     if (capturing != hipStreamCaptureStatusNone) return NERF_ERR_ARG;
     if (!plan->chunks) return NERF_OK;
     StepArgs a = {};
-    a.tensors = plan->d_tensors;
     a.chunks = plan->d_chunks;
-    a.chunk = plan->chunk;
     a.lr = learning_rate;
     a.root_c2t = sqrtf(1.0f - powf(plan->beta2, (float)step));
     a.c1t = 1.0f - powf(plan->beta1, (float)step);
@@ -540,10 +664,20 @@ int nerf_adamw_step(NerfAdamw* plan, int step, float learning_rate, float grad_d
     z ^= z >> 31;
     a.key = (unsigned)(z ^ (z >> 32));
     ProfScope prof(K_ADAMW, plan->bytes);
-    if (plan->state_bits == 8)
-        hipLaunchKernelGGL(adamw8_kernel, dim3(plan->chunks), dim3(256), 0, stream(), a, seed != 0);
-    else
-        hipLaunchKernelGGL(adamw32_kernel, dim3(plan->chunks), dim3(256), 0, stream(), a);
+    const dim3 grid(plan->chunks * PIECES), block(256);
+    const bool stream_past = plan->bytes > STREAM_BYTES;
+#define STEP(KERNEL) hipLaunchKernelGGL(KERNEL, grid, block, 0, stream(), a)
+    if (plan->state_bits == 32) {
+        if (stream_past) STEP(adamw32_kernel<true>);
+        else STEP(adamw32_kernel<false>);
+    } else if (seed) {
+        if (stream_past) STEP((adamw8_kernel<true, true>));
+        else STEP((adamw8_kernel<true, false>));
+    } else {
+        if (stream_past) STEP((adamw8_kernel<false, true>));
+        else STEP((adamw8_kernel<false, false>));
+    }
+#undef STEP
     return hipGetLastError() == hipSuccess ? NERF_OK : NERF_ERR_HIP;
 }
 
@@ -551,17 +685,24 @@ int nerf_adamw_read_states(NerfAdamw* plan, unsigned short* d_m, unsigned short*
     if (!plan || plan->state_bits != 8 || (!d_m && !d_root_v) || (((uintptr_t)d_m | (uintptr_t)d_root_v) & 1) || !plan_usable(plan))
         return NERF_ERR_ARG;
     if (!plan->chunks) return NERF_OK;
-    hipLaunchKernelGGL(read_states_kernel, dim3(plan->chunks), dim3(256), 0, stream(), plan->d_tensors, plan->d_chunks,
-                       plan->chunk, d_m, d_root_v);
+    if (plan->bytes > STREAM_BYTES)
+        hipLaunchKernelGGL(read_states_kernel<true>, dim3(plan->chunks), dim3(256), 0, stream(), plan->d_chunks, d_m, d_root_v);
+    else
+        hipLaunchKernelGGL(read_states_kernel<false>, dim3(plan->chunks), dim3(256), 0, stream(), plan->d_chunks, d_m, d_root_v);
     return hipGetLastError() == hipSuccess ? NERF_OK : NERF_ERR_HIP;
 }
 
 int nerf_grad_norm(NerfAdamw* plan, float grad_div, float* d_norm) {
     if (!plan || !d_norm || ((uintptr_t)d_norm & 3) || !(grad_div > 0.0f && grad_div < INFINITY) || !plan_usable(plan)) return NERF_ERR_ARG;
-    const unsigned blocks = std::max(1u, std::min(plan->chunks, NORM_BLOCKS));
+    // A piece to a wavefront up to one workgroup per CU, two workgroups for long lists: every workgroup adds 10 ns for its
+    // ticket, every further round of pieces the time of a read.  134 million bf16 elements take 94.9, 55.5, 46.9 and 49.7 us
+    // with at most 128, 256, 512 and 1024 workgroups (5.7 TB/s), 16 million in fp32 13.2, 13.8, 15.4 and 19.3 us, 603 136
+    // (37 workgroups) 4.9 us; workgroups of four wavefronts took 60 and 16.7 us at their best.
+    const unsigned pieces = plan->chunks * PIECES, most = pieces < 65536 ? 256 : NORM_BLOCKS;
+    const unsigned blocks = std::max(1u, std::min((pieces + NORM_WAVES - 1) / NORM_WAVES, most));
     ProfScope prof(K_GRAD_NORM, plan->grad_bytes);
-    hipLaunchKernelGGL(grad_norm_kernel, dim3(blocks), dim3(256), 0, stream(), plan->d_tensors, plan->d_chunks, plan->chunks,
-                       plan->chunk, plan->d_partial, plan->d_ticket, grad_div, d_norm);
+    hipLaunchKernelGGL(grad_norm_kernel, dim3(blocks), dim3(64 * NORM_WAVES), 0, stream(), plan->d_chunks, plan->chunks * PIECES, plan->d_partial,
+                       plan->d_ticket, grad_div, d_norm);
     return hipGetLastError() == hipSuccess ? NERF_OK : NERF_ERR_HIP;
 }
 
