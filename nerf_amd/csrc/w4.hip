@@ -6,6 +6,8 @@
 #include "common.hpp"
 #include "../../include/nerf_amd.h"
 
+#include <math.h>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -36,27 +38,37 @@ __device__ __forceinline__ void values8(unsigned c, float* v) {
     v[4] = d[0]; v[5] = d[1]; v[6] = e[0]; v[7] = e[1];
 }
 
-// ---- quantize -------------------------------------------------------------------------------------------
-// A thread takes eight consecutive columns of a row; the 4, 8 or 16 threads of a group are neighbours in a row of
-// sixteen lanes.  `per_row` threads (whole groups) belong to a row.
+// ---- quantize and dequantize ----------------------------------------------------------------------------
+constexpr unsigned SLAB = 0x40000000u;  // pieces of a slab of rows (gridDim.y of them): their numbers fit 32 bits
+
+// piece number `id` of a slab: its row (of all), or rows if there is none, and its place in the row; `per_row` to a row
+__device__ __forceinline__ long piece_of(unsigned id, unsigned per_row, int rows, unsigned& place) {
+    const unsigned in_slab = id / per_row, slab_rows = SLAB / per_row;
+    place = id - in_slab * per_row;
+    const long row = (long)blockIdx.y * slab_rows + in_slab;
+    return in_slab < slab_rows && row < rows ? row : rows;
+}
+
+// A thread takes eight consecutive columns of a row; the 4, 8 or 16 threads of a group are neighbours in a row of sixteen
+// lanes (a row of W has whole groups of threads).
 template <int GROUP>
 __global__ __launch_bounds__(256) void quantize_w4_kernel(const float* __restrict__ src, long ld, int rows, int cols,
                                                           unsigned per_row, unsigned char* __restrict__ codes,
                                                           long row_bytes, unsigned short* __restrict__ scales, int groups) {
-    const unsigned id = blockIdx.x * 256 + threadIdx.x;
-    const unsigned slab_row = id / per_row, piece = id - slab_row * per_row;
-    const long row = (long)blockIdx.y * (0x40000000u / per_row) + slab_row;
-    const bool live = row < rows && slab_row < 0x40000000u / per_row;
-    const int col = (int)piece * 8;
+    unsigned place;
+    const long row = piece_of(blockIdx.x * 256 + threadIdx.x, per_row, rows, place);
+    const int col = (int)place * 8;
     float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (live) {
+    if (row < rows) {
         const float* p = src + row * ld + col;
         if (col + 8 <= cols) {
             const f32x4u a = *reinterpret_cast<const f32x4u*>(p), b = *reinterpret_cast<const f32x4u*>(p + 4);
 #pragma unroll
             for (int k = 0; k < 4; k++) { x[k] = a[k]; x[k + 4] = b[k]; }
         } else {
-            for (int k = 0; k < 8 && col + k < cols; k++) x[k] = p[k];
+#pragma unroll
+            for (int k = 0; k < 7; k++)
+                if (col + k < cols) x[k] = p[k];
         }
     }
     unsigned top = 0;  // of the magnitudes' bits: infinities and NaN come out on top
@@ -71,40 +83,51 @@ __global__ __launch_bounds__(256) void quantize_w4_kernel(const float* __restric
     unsigned s = __builtin_bit_cast(unsigned, largest * (1.0f / 6.0f)) >> 16;
     s += 6.0f * bf16_to_f32((unsigned short)s) < largest;
     const bool bad = top >= 0x7F800000u;
-    const float scale = bad ? 0.0f : bf16_to_f32((unsigned short)s);
-    if (!live) return;
-    // steps between codes, where the value of the border (a multiple of the scale) is exact; a tie takes the even code
+    if (row >= rows) return;
+    // The borders between codes are multiples of the scale and exact in fp32; a tie takes the even code.  Which side of three
+    // borders a weight is on gives the three bits.  Without a scale (a group of zeros, or one that is not finite) every
+    // border is out of reach.
+    const float scale = bad || top == 0 ? INFINITY : bf16_to_f32((unsigned short)s);
+    const float b1 = 0.25f * scale, b2 = 0.75f * scale, b3 = 1.25f * scale, b4 = 1.75f * scale, b5 = 2.5f * scale, b6 = 3.5f * scale,
+                b7 = 5.0f * scale;
     unsigned word = 0;
 #pragma unroll
     for (int k = 0; k < 8; k++) {
-        const float a = fabsf(x[k]);
-        unsigned c = (a > 0.25f * scale) + (a >= 0.75f * scale) + (a > 1.25f * scale) + (a >= 1.75f * scale) +
-                     (a > 2.5f * scale) + (a >= 3.5f * scale) + (a > 5.0f * scale);
-        if (bad || top == 0) c = 0;
+        const float a = bad ? 0.0f : fabsf(x[k]);
+        const bool four = a >= b4, two = a >= (four ? b6 : b2);
+        const float lower = four ? b5 : b1, upper = four ? b7 : b3;
+        const bool one = a > (two ? upper : lower);
+        unsigned c = four ? 4u : 0u;
+        c = c + (two ? 2u : 0u) + (one ? 1u : 0u);
         if (c && x[k] < 0.0f) c |= 8;
         word |= c << (4 * k);
     }
-    if ((long)piece * 4 < row_bytes) *reinterpret_cast<unsigned*>(codes + row * row_bytes + (long)piece * 4) = word;
-    if (piece % (GROUP / 8) == 0) scales[row * groups + piece / (GROUP / 8)] = bad ? 0x7FC0 : (unsigned short)s;
+    if ((long)place * 4 < row_bytes) *reinterpret_cast<unsigned*>(codes + row * row_bytes + (long)place * 4) = word;
+    if (place % (GROUP / 8) == 0) scales[row * groups + place / (GROUP / 8)] = bad ? 0x7FC0 : (unsigned short)s;
 }
 
+// A thread does two pieces of four consecutive columns, so that a wavefront writes whole lines, and past the caches: a
+// half-written line does not wait for its other half (8192 x 8192: 42 us = 7.2 TB/s; through the caches 62, and 104 where a
+// thread's eight columns went out in two halves past them).
 __global__ __launch_bounds__(256) void dequantize_w4_kernel(const unsigned char* __restrict__ codes, long row_bytes,
                                                             const unsigned short* __restrict__ scales, int groups, int group,
                                                             int rows, int cols, unsigned per_row, float* __restrict__ dst, long ld) {
-    const unsigned id = blockIdx.x * 256 + threadIdx.x;
-    const unsigned slab_row = id / per_row, piece = id - slab_row * per_row;
-    const long row = (long)blockIdx.y * (0x40000000u / per_row) + slab_row;
-    if (row >= rows || slab_row >= 0x40000000u / per_row) return;
-    const int col = (int)piece * 8;
-    const float scale = bf16_to_f32(scales[row * groups + col / group]);
-    float v[8];
-    values8(*reinterpret_cast<const unsigned*>(codes + row * row_bytes + (long)piece * 4), v);
-    float* p = dst + row * ld + col;
-    if (col + 8 <= cols) {
-        *reinterpret_cast<f32x4u*>(p) = f32x4u{v[0] * scale, v[1] * scale, v[2] * scale, v[3] * scale};
-        *reinterpret_cast<f32x4u*>(p + 4) = f32x4u{v[4] * scale, v[5] * scale, v[6] * scale, v[7] * scale};
-    } else {
-        for (int k = 0; k < 8 && col + k < cols; k++) p[k] = v[k] * scale;
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+        unsigned place;
+        const long row = piece_of(blockIdx.x * 512 + u * 256 + threadIdx.x, per_row, rows, place);
+        if (row >= rows) continue;
+        const int col = (int)place * 4;
+        const float scale = bf16_to_f32(scales[row * groups + col / group]);
+        const unsigned c = *reinterpret_cast<const unsigned short*>(codes + row * row_bytes + (long)place * 2);
+        const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 1);
+        const f32x4u v = {a[0] * scale, a[1] * scale, b[0] * scale, b[1] * scale};
+        float* p = dst + row * ld + col;
+        if (col + 4 <= cols) __builtin_nontemporal_store(v, reinterpret_cast<f32x4u*>(p));
+        else
+#pragma unroll
+            for (int k = 0; k < 3; k++)
+                if (col + k < cols) p[k] = v[k];
     }
 }
 
@@ -728,11 +751,11 @@ bool group_ok(int group) { return group == 32 || group == 64 || group == 128; }
 bool type_ok(int t) { return t == NERF_TYPE_F32 || t == NERF_TYPE_BF16; }
 int ceil_div(int a, int b) { return a / b + (a % b != 0); }
 
-// launch shape of the two conversions: rows in slabs whose threads fit 32 bits
-dim3 piece_grid(int rows, unsigned per_row) {
-    const unsigned slab = 0x40000000u / per_row;
+// launch shape of the two conversions, `block` pieces to a workgroup
+dim3 piece_grid(int rows, unsigned per_row, unsigned block) {
+    const unsigned slab = SLAB / per_row;
     const unsigned in_slab = std::min((unsigned)rows, slab);
-    return dim3((unsigned)(((unsigned long long)in_slab * per_row + 255) / 256), ((unsigned)rows + slab - 1) / slab);
+    return dim3((unsigned)(((unsigned long long)in_slab * per_row + block - 1) / block), ((unsigned)rows + slab - 1) / slab);
 }
 
 }  // namespace
@@ -753,13 +776,9 @@ int nerf_quantize_w4(const float* d_src, long ld_src, int rows, int cols, int gr
     const unsigned per_row = (unsigned)groups * (unsigned)(group / 8);
     const long row_bytes = (long)nerf_w4_row_bytes(cols);
     ProfScope prof(K_QUANTIZE_W4, (double)rows * cols * 4.5);
-#define QUANTIZE(G)                                                                                                        \
-    hipLaunchKernelGGL((quantize_w4_kernel<G>), piece_grid(rows, per_row), dim3(256), 0, stream(), d_src, ld_src, rows, cols, \
-                       per_row, d_codes, row_bytes, d_scales, groups)
-    if (group == 32) QUANTIZE(32);
-    else if (group == 64) QUANTIZE(64);
-    else QUANTIZE(128);
-#undef QUANTIZE
+    const auto kernel = group == 32 ? quantize_w4_kernel<32> : group == 64 ? quantize_w4_kernel<64> : quantize_w4_kernel<128>;
+    hipLaunchKernelGGL(kernel, piece_grid(rows, per_row, 256), dim3(256), 0, stream(), d_src, ld_src, rows, cols, per_row, d_codes, row_bytes,
+                       d_scales, groups);
     return hipGetLastError() == hipSuccess ? NERF_OK : NERF_ERR_HIP;
 }
 
@@ -768,10 +787,10 @@ int nerf_dequantize_w4(const unsigned char* d_codes, const unsigned short* d_sca
     if (!d_dst || !d_codes || !d_scales || rows <= 0 || cols <= 0 || ld_dst < cols || !group_ok(group) ||
         ((uintptr_t)d_dst & 3) || ((uintptr_t)d_codes & 15) || ((uintptr_t)d_scales & 1))
         return NERF_ERR_ARG;
-    const unsigned per_row = (unsigned)ceil_div(cols, 8);
+    const unsigned per_row = (unsigned)ceil_div(cols, 4);
     ProfScope prof(K_QUANTIZE_W4, (double)rows * cols * 4.5);
-    hipLaunchKernelGGL(dequantize_w4_kernel, piece_grid(rows, per_row), dim3(256), 0, stream(), d_codes,
-                       (long)nerf_w4_row_bytes(cols), d_scales, ceil_div(cols, group), group, rows, cols, per_row, d_dst, ld_dst);
+    hipLaunchKernelGGL(dequantize_w4_kernel, piece_grid(rows, per_row, 512), dim3(256), 0, stream(), d_codes, (long)nerf_w4_row_bytes(cols),
+                       d_scales, ceil_div(cols, group), group, rows, cols, per_row, d_dst, ld_dst);
     return hipGetLastError() == hipSuccess ? NERF_OK : NERF_ERR_HIP;
 }
 
