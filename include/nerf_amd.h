@@ -186,6 +186,7 @@ int nerf_grad_norm(NerfAdamw* plan, float grad_div, float* d_norm);
  * sign and magnitude 0, 0.5, 1, 1.5, 2, 3, 4, 6 (codes 0..7; plus 8 for negative) -- and one bf16 scale per `group`
  * (32, 64 or 128) consecutive columns of a row, [rows][ceil(cols / group)].  A weight is code value * scale. ---- */
 size_t nerf_w4_row_bytes(int cols); /* 16 bytes per 32 columns, rounded up */
+#define NERF_W4_MAX_DIM (1 << 30)   /* columns (K) of a matrix, and rows (N) of one that is multiplied with */
 /* scale = the smallest bf16 with 6 scale >= largest |weight| of the group, codes to nearest with ties to the even
  * code.  A group that holds a weight that is not finite gets a NaN scale.  Rows of d_src are ld_src >= cols floats
  * apart; codes behind the last column are zero.  d_codes must be 16-byte aligned. */

@@ -358,6 +358,11 @@ __global__ __launch_bounds__(64 * WAVES) void gemv_w4_kernel(const W4Args a, con
 // (16 x 16 x 32), so that a step's 32 columns lie in one group and the sum over a group takes one scale.  Columns of
 // workgroups start at different chunks of a slice: rows of W are often a power of two apart, and workgroups that walk
 // them in step would all ask the same few memory channels.
+//   Times (groups of 64): 24 x 4100 x 4090 16.2 us (bf16 12.6), of which W's bytes are 1.4 us, two launches 5, and the rest a
+// chain that is too short to overlap: X arrives and is split, W arrives, matrix instructions, sums written and read again.
+// 16 x 16384 x 8192 29.3 us = 2.4 TB/s of W (every workgroup of 256 columns reads as many bytes of X from the L2 as half its
+// own of W, and each wavefront reads all of them again from LDS); 64 x 16384 x 8192 in bf16 38.7 us = 443 TFLOP/s.  Eight
+// chunks of W ahead instead of DEPTH, or four wavefronts instead of eight, measured the same to 15 % slower.
 // eight codes as eight bf16
 __device__ __forceinline__ bf16x8 values8_bf16(unsigned c) {
     const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, 1.0f, 1);
@@ -370,13 +375,18 @@ __device__ __forceinline__ unsigned upper_halves(unsigned lo, unsigned hi) { ret
 
 // the upper, middle and lower 8 significant bits of an fp32 number, each as the upper half of a word (a bf16 number)
 __device__ __forceinline__ void split3(unsigned x, unsigned& hi, unsigned& mid, unsigned& lo) {
-    // infinity less itself would be NaN: what is not finite goes in the first part alone
-    const bool special = (x & 0x7F800000u) == 0x7F800000u;
-    const float rest = special ? 0.0f : __builtin_bit_cast(float, x) - __builtin_bit_cast(float, x & 0xFFFF0000u);
+    const float rest = __builtin_bit_cast(float, x) - __builtin_bit_cast(float, x & 0xFFFF0000u);
+    hi = x;
     mid = __builtin_bit_cast(unsigned, rest);
     lo = __builtin_bit_cast(unsigned, rest - __builtin_bit_cast(float, mid & 0xFFFF0000u));
-    // a NaN whose upper half alone would read as infinity stays a NaN
+}
+// the same for a number that may not be finite: infinity less itself would be NaN, and a NaN cut off could read as infinity,
+// so these go in the first part alone
+__device__ __forceinline__ void split3_any(unsigned x, unsigned& hi, unsigned& mid, unsigned& lo) {
+    split3(x, hi, mid, lo);
+    if ((x & 0x7F800000u) != 0x7F800000u) return;
     hi = (x & 0x7FFFFFFFu) > 0x7F800000u ? 0x7FC00000u : x;
+    mid = lo = 0;
 }
 
 // Eight consecutive values of a row of X as they lie in memory, and as one or three operands of eight bf16
@@ -401,8 +411,17 @@ struct Piece {
             o[0] = v[0];
         } else {
             unsigned hi[8], mid[8], lo[8];
+            float none = 0.0f;  // of finite numbers, times zero
 #pragma unroll
-            for (int k = 0; k < 8; k++) split3(v[k / 4][k % 4], hi[k], mid[k], lo[k]);
+            for (int k = 0; k < 8; k++) {
+                const unsigned x = v[k / 4][k % 4];
+                split3(x, hi[k], mid[k], lo[k]);
+                none = __builtin_fmaf(__builtin_bit_cast(float, x), 0.0f, none);
+            }
+            if (none != 0.0f) {
+#pragma unroll
+                for (int k = 0; k < 8; k++) split3_any(v[k / 4][k % 4], hi[k], mid[k], lo[k]);
+            }
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 o[0][k] = upper_halves(hi[2 * k], hi[2 * k + 1]);
@@ -422,9 +441,10 @@ __device__ __forceinline__ u32x4 transpose4(u32x4 d) {
     return u32x4{c[0], c[1], e[0], e[1]};
 }
 
-// A chunk of one of a lane's rows of W: its codes, and the scales of the chunk's groups as they lie in memory.  In the last
-// chunk of a row that is no multiple of 128 long, a unit past the row's end is the last one again (X is zero there), and
-// a group past the end has the scale zero.
+// A chunk of one of a lane's rows of W as it lies in memory: its codes, and the scales of its groups.  In the last chunk of
+// a row that is no multiple of 128 long, a unit past the row's end is the last one again (X is zero there), and the
+// scales are those of the row's last groups: `past` bits too far up, above which there is zero for the groups that are
+// not there.  Nothing is done to what is loaded before it is used, or the load would be waited for.
 template <int GROUP>
 struct Chunk4 {
     static constexpr int GROUPS = 128 / GROUP;
@@ -436,15 +456,13 @@ struct Chunk4 {
                                          int groups) {
         codes = *reinterpret_cast<const u32x4*>(codes_row + (long)min(unit, units - 1) * 16);
         if (groups >= GROUPS) {
-            const int start = min(first, groups - GROUPS), past = (first - start) * 16;  // bits to drop
-            const unsigned short* p = scales_row + start;
+            const unsigned short* p = scales_row + min(first, groups - GROUPS);
             if constexpr (GROUP == 32) {
                 const u32x2u s = *reinterpret_cast<const u32x2u*>(p);
-                const unsigned long long both = ((unsigned long long)s[1] << 32 | s[0]) >> past;
-                scales[0] = (unsigned)both;
-                scales[1] = (unsigned)(both >> 32);
+                scales[0] = s[0];
+                scales[1] = s[1];
             } else if constexpr (GROUP == 64) {
-                scales[0] = *reinterpret_cast<const u32u*>(p) >> past;
+                scales[0] = *reinterpret_cast<const u32u*>(p);
             } else {
                 scales[0] = *p;
             }
@@ -453,8 +471,23 @@ struct Chunk4 {
             if constexpr (GROUP == 32) scales[1] = groups > 2 ? scales_row[2] : 0u;
         }
     }
-    __device__ __forceinline__ float scale(int g) const {  // of the chunk's group g
-        return __builtin_bit_cast(float, g & 1 ? scales[g / 2] & 0xFFFF0000u : scales[g / 2] << 16);
+    // the scales of the chunk's groups
+    __device__ __forceinline__ void take(int first, int groups, float* s) const {
+        const int past = max(0, first - (groups - GROUPS)) * (groups >= GROUPS ? 16 : 0);
+        if constexpr (GROUP == 32) {
+            const unsigned long long all = ((unsigned long long)scales[1] << 32 | scales[0]) >> past;
+            const unsigned lo = (unsigned)all, hi = (unsigned)(all >> 32);
+            s[0] = __builtin_bit_cast(float, lo << 16);
+            s[1] = __builtin_bit_cast(float, lo & 0xFFFF0000u);
+            s[2] = __builtin_bit_cast(float, hi << 16);
+            s[3] = __builtin_bit_cast(float, hi & 0xFFFF0000u);
+        } else if constexpr (GROUP == 64) {
+            const unsigned all = scales[0] >> past;
+            s[0] = __builtin_bit_cast(float, all << 16);
+            s[1] = __builtin_bit_cast(float, all & 0xFFFF0000u);
+        } else {
+            s[0] = __builtin_bit_cast(float, scales[0] << 16);
+        }
     }
 };
 
@@ -464,6 +497,7 @@ struct GemmShape {
     float* partial;    // [parts][M][N], or null: one part, stored to Y
 };
 
+constexpr int CUS = 256;
 constexpr int DEPTH = 2;  // chunks of W on their way to a wavefront
 
 // chunks of a slice: with this many, a slice of R MT rows is four pieces of eight columns for each thread
@@ -550,7 +584,7 @@ __global__ __launch_bounds__(64 * WAVES) void gemm_w4_kernel(const W4Args a, con
                 if (col < a.K) {
                     const long from = (m0 + r) * a.ldx + col;
                     if constexpr (XBF) h[0] = (unsigned)((const unsigned short*)a.X)[from] << 16;
-                    else split3(((const unsigned*)a.X)[from], h[0], h[1], h[2]);
+                    else split3_any(((const unsigned*)a.X)[from], h[0], h[1], h[2]);
                 }
                 char* at = at_piece(r, ragged / 8 - base * 16) + (q % 8) * 2;
 #pragma unroll
@@ -562,15 +596,21 @@ __global__ __launch_bounds__(64 * WAVES) void gemm_w4_kernel(const W4Args a, con
     const char* xlane = lds + (lj * R + min(ln, R - 1)) * 16;
 
     Chunk4<GROUP> w[DEPTH][NT];
+    load_x(first);  // before W: loads come back in their order, and X is waited for first
     if (turns_all) {
 #pragma unroll
         for (int d = 0; d < DEPTH; d++) load(w[d], d);
     }
     auto chunk = [&](const Chunk4<GROUP>* w, int turn, int base) {
-        const char* xs = xlane + (chunk_of(turn) - base) * (4 * STEP_BYTES);
+        const int c = chunk_of(turn);
+        const char* xs = xlane + (c - base) * (4 * STEP_BYTES);
         u32x4 codes[NT];
+        float scales[NT][128 / GROUP];
 #pragma unroll
-        for (int t = 0; t < NT; t++) codes[t] = transpose4(w[t].codes);
+        for (int t = 0; t < NT; t++) {
+            codes[t] = transpose4(w[t].codes);
+            w[t].take(c * (128 / GROUP), a.groups, scales[t]);
+        }
         f32x4 part[MT][NT];
 #pragma unroll
         for (int s = 0; s < 4; s++) {
@@ -583,7 +623,7 @@ __global__ __launch_bounds__(64 * WAVES) void gemm_w4_kernel(const W4Args a, con
 #pragma unroll
             for (int t = 0; t < NT; t++) {
                 const bf16x8 v = values8_bf16(codes[t][s]);
-                const float scale = w[t].scale(s / STEPS);
+                const float scale = scales[t][s / STEPS];
 #pragma unroll
                 for (int i = 0; i < MT; i++) {
                     if (s % STEPS == 0) part[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -601,7 +641,7 @@ __global__ __launch_bounds__(64 * WAVES) void gemm_w4_kernel(const W4Args a, con
     int turn = 0;
     for (int base = first - SLICE; base < end; base += SLICE) {  // the first time round there is no slice yet
         const bool more = base + SLICE < end;
-        if (more) load_x(base + SLICE);
+        if (more && base >= first) load_x(base + SLICE);
         if (base >= first) {
             const int stop = min(turns_all, turn + (1 << log_turns));
             // a whole slice has a multiple of DEPTH turns
@@ -650,43 +690,62 @@ __global__ __launch_bounds__(64 * WAVES) void gemm_w4_kernel(const W4Args a, con
     }
 }
 
-// the parts of a split contraction, added in their order
+// the parts of a split contraction, added in their order; four columns to a thread, a row of Y to gridDim.y
 __global__ __launch_bounds__(256) void join_w4_kernel(const W4Args a, const float* partial, int parts) {
-    const long id = (long)blockIdx.x * 256 + threadIdx.x, size = (long)a.M * a.N;
-    if (id >= size) return;
-    float y = partial[id];
-    for (int p = 1; p < parts; p++) y += partial[p * size + id];
-    const long m = id / a.N;
-    store_y(a, m * a.ldy + (id - m * a.N), y);
+    const int n = (blockIdx.x * 256 + threadIdx.x) * 4;
+    const long m = blockIdx.y, size = (long)a.M * a.N;
+    if (n >= a.N) return;
+    const float* p = partial + m * a.N + n;
+    const int columns = min(4, a.N - n);
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+    if (columns == 4) {
+        y = *reinterpret_cast<const f32x4u*>(p);
+#pragma unroll 4
+        for (int k = 1; k < parts; k++) {
+            const f32x4 z = *reinterpret_cast<const f32x4u*>(p + k * size);
+#pragma unroll
+            for (int r = 0; r < 4; r++) y[r] += z[r];
+        }
+    } else {
+        for (int k = 0; k < parts; k++)
+#pragma unroll
+            for (int r = 0; r < 3; r++)
+                if (r < columns) y[r] = k ? y[r] + p[k * size + r] : p[r];
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+        if (r < columns) store_y(a, m * a.ldy + n + r, y[r]);
 }
 
 struct GemmPlan {
     int r, mt, nt, log_kw, parts, split_chunks;
 };
 
-#ifdef TUNE
-}}
-extern "C" { int tune[8]; }
-namespace nerf { namespace {
-#endif
-
+// Which wavefronts share what (times: groups of 64, X in fp32 unless it says bf16):
+//   Rows of X to a workgroup: all of them up to 64, so that W is read and converted once.
+//   Columns of a wavefront: 32 where there are many, since a tile of X read from LDS then serves two tiles of W: 16 x 16384
+// x 8192 takes 30.2 us with 32 and 33.9 with 16, 64 x 16384 x 8192 62.8 and 77.4 (bf16: 39.4 and 38.0).  But 16 where only
+// that gives every CU a workgroup of its own: 64 x 32768 x 1024 takes 25.2 us with 16 and 29.7 with 32.
+//   Wavefronts along the contraction, which cost nothing but a narrower workgroup, so that X is read more often.  Up to
+// four rows X is small, and they go up to a workgroup for each CU: 3 x 4096 x 4096 takes 6.4, 8.6 and 33 us with 8, 4 and 1.
+// Else they go up to 64 workgroups: 16 x 4096 x 4096 takes 10.9 us with 2 and four parts, 12.3 with 4 and three, 11.5 with 1
+// and eight.
+//   Parts of the contraction, each in workgroups of its own, fill the CUs then.  They are joined by a second kernel, about
+// 3 us, and a part has at least a slice of X: 16 x 256 x 16384 in bf16 takes 9.8 us with 16 parts, 11.2 with 32 or 8.
 GemmPlan plan_gemm(int M, int N, int K) {
     GemmPlan p = {};
     const int chunks = K / 128 + (K % 128 != 0);
     p.r = M <= 4 ? 4 : 16;
     p.mt = M <= 16 ? 1 : M <= 32 ? 2 : 4;
-    p.nt = N >= 8192 ? 2 : 1;
     const int slice = slice_chunks(p.r, p.mt);
     const long m_blocks = (M + p.r * p.mt - 1L) / (p.r * p.mt);
-    auto blocks = [&] { return ((long)N + 16 * p.nt * (WAVES >> p.log_kw) - 1) / (16 * p.nt * (WAVES >> p.log_kw)) * m_blocks; };
-    while (blocks() < 128 && (slice >> p.log_kw) > DEPTH && (chunks >> p.log_kw) > 1 && p.log_kw < 3) p.log_kw++;
-    p.parts = (int)std::max(1L, std::min(std::min(16L, chunks / 4L), 256 / blocks()));
-#ifdef TUNE
-    if (tune[0]) p.nt = tune[0];
-    if (tune[1]) p.log_kw = tune[1] - 1;
-    if (tune[2]) p.parts = tune[2];
-    while (p.log_kw && ((slice >> p.log_kw) < DEPTH || (chunks >> p.log_kw) < 1)) p.log_kw--;
-#endif
+    auto blocks = [&](int nt) {
+        const int columns = 16 * nt * (WAVES >> p.log_kw);
+        return ((long)N + columns - 1) / columns * m_blocks;
+    };
+    p.nt = N >= 8192 && (blocks(2) >= CUS || blocks(1) < CUS) ? 2 : 1;
+    while (blocks(p.nt) < (p.r == 4 ? CUS : CUS / 4) && (slice >> p.log_kw) > DEPTH && (chunks >> p.log_kw) > 1 && p.log_kw < 3) p.log_kw++;
+    p.parts = (int)std::max(1L, std::min(std::min(64L, (long)chunks / (8 / p.mt)), CUS / blocks(p.nt)));
     p.split_chunks = (chunks + p.parts - 1) / p.parts;
     if (p.parts > 1 && p.split_chunks > slice) p.split_chunks = (p.split_chunks + slice - 1) / slice * slice;
     p.parts = (chunks + p.split_chunks - 1) / p.split_chunks;
@@ -699,13 +758,18 @@ hipError_t launch_gemm(const W4Args& a, const GemmPlan& p, float* partial) {
     const size_t x_bytes = (size_t)std::min(slice_chunks(R, MT), p.split_chunks) * 4 * (PARTS * MT * R * 64 + 16);
     const size_t bytes = std::max(x_bytes, (size_t)WAVES * NT * 64 * 16);
     const long columns = 16L * NT * (WAVES >> p.log_kw);
-    const dim3 grid((unsigned)((a.N + columns - 1) / columns), (unsigned)((a.M + R * MT - 1L) / (R * MT)), (unsigned)p.parts);
     const GemmShape shape = {p.log_kw, p.split_chunks, p.parts > 1 ? partial : nullptr};
-    hipLaunchKernelGGL((gemm_w4_kernel<R, MT, NT, XBF, GROUP>), grid, dim3(64 * WAVES), bytes, stream(), a, shape);
-    if (p.parts > 1) {
-        const long size = (long)a.M * a.N;
-        hipLaunchKernelGGL(join_w4_kernel, dim3((unsigned)((size + 255) / 256)), dim3(256), 0, stream(), a, partial, p.parts);
+    constexpr long MOST = 65535L * R * MT;  // rows of a launch: gridDim.y has 16 bits
+    for (long m = 0; m < a.M; m += MOST) {
+        W4Args some = a;
+        some.M = (int)std::min(MOST, a.M - m);
+        some.X = (const char*)a.X + m * a.ldx * (XBF ? 2 : 4);
+        some.Y = (char*)a.Y + m * a.ldy * (a.y_bf16 ? 2 : 4);
+        const dim3 grid((unsigned)((a.N + columns - 1) / columns), (unsigned)((some.M + R * MT - 1L) / (R * MT)), (unsigned)p.parts);
+        hipLaunchKernelGGL((gemm_w4_kernel<R, MT, NT, XBF, GROUP>), grid, dim3(64 * WAVES), bytes, stream(), some, shape);
     }
+    if (p.parts > 1)
+        hipLaunchKernelGGL(join_w4_kernel, dim3((unsigned)((a.N + 1023L) / 1024), (unsigned)a.M), dim3(256), 0, stream(), a, partial, p.parts);
     return hipGetLastError();
 }
 template <int R, int MT, int NT>
@@ -736,9 +800,6 @@ hipError_t launch_gemv(const W4Args& a) {
     // (256 workgroups) and 15.1 with 16; 1 x 512 x 512 takes 3.1 us with 2 and 5.0 with 8.
     const long row = (64 >> g.log_lanes) * (WAVES >> g.log_kw);
     while (g.loads < 32 && g.loads * row < 4096 && a.N / (g.loads * row) >= (a.x_bf16 ? 512 : 256) + 1) g.loads *= 2;
-#ifdef TUNE
-    if (tune[4]) g.loads = tune[4];
-#endif
     const long block_rows = g.loads * row;
     const dim3 grid((unsigned)((a.N + block_rows - 1) / block_rows));
     const size_t bytes = (a.x_bf16 ? 0 : (size_t)M * 8 * g.stride) + (size_t)block_rows * (M << g.log_kw) * sizeof(float);
@@ -769,7 +830,7 @@ size_t nerf_w4_row_bytes(int cols) { return cols > 0 ? ((size_t)cols + 31) / 32 
 
 int nerf_quantize_w4(const float* d_src, long ld_src, int rows, int cols, int group, unsigned char* d_codes,
                      unsigned short* d_scales) {
-    if (!d_src || !d_codes || !d_scales || rows <= 0 || cols <= 0 || ld_src < cols || !group_ok(group) ||
+    if (!d_src || !d_codes || !d_scales || rows <= 0 || cols <= 0 || cols > NERF_W4_MAX_DIM || ld_src < cols || !group_ok(group) ||
         ((uintptr_t)d_src & 3) || ((uintptr_t)d_codes & 15) || ((uintptr_t)d_scales & 1))
         return NERF_ERR_ARG;
     const int groups = ceil_div(cols, group);
@@ -784,7 +845,7 @@ int nerf_quantize_w4(const float* d_src, long ld_src, int rows, int cols, int gr
 
 int nerf_dequantize_w4(const unsigned char* d_codes, const unsigned short* d_scales, int rows, int cols, int group,
                        float* d_dst, long ld_dst) {
-    if (!d_dst || !d_codes || !d_scales || rows <= 0 || cols <= 0 || ld_dst < cols || !group_ok(group) ||
+    if (!d_dst || !d_codes || !d_scales || rows <= 0 || cols <= 0 || cols > NERF_W4_MAX_DIM || ld_dst < cols || !group_ok(group) ||
         ((uintptr_t)d_dst & 3) || ((uintptr_t)d_codes & 15) || ((uintptr_t)d_scales & 1))
         return NERF_ERR_ARG;
     const unsigned per_row = (unsigned)ceil_div(cols, 4);
@@ -795,8 +856,7 @@ int nerf_dequantize_w4(const unsigned char* d_codes, const unsigned short* d_sca
 }
 
 size_t nerf_gemm_w4_workspace(int M, int N, int K) {
-    if (M <= 0 || N <= 0 || K <= 0) return 0;
-    if (M <= 2) return 0;
+    if (M <= 2 || N <= 0 || K <= 0) return 0;
     const GemmPlan p = plan_gemm(M, N, K);
     return p.parts > 1 ? (size_t)p.parts * M * N * sizeof(float) : 0;
 }
@@ -804,7 +864,7 @@ size_t nerf_gemm_w4_workspace(int M, int N, int K) {
 int nerf_gemm_w4(const void* d_X, int x_type, long ldx, const unsigned char* d_codes, const unsigned short* d_scales,
                  int group, void* d_Y, int y_type, long ldy, int M, int N, int K, int epilogue, void* d_workspace,
                  size_t workspace_bytes) {
-    if (!d_X || !d_codes || !d_scales || !d_Y || M <= 0 || N <= 0 || K <= 0 || ldx < K || ldy < N || !group_ok(group) ||
+    if (!d_X || !d_codes || !d_scales || !d_Y || M <= 0 || N <= 0 || K <= 0 || N > NERF_W4_MAX_DIM || K > NERF_W4_MAX_DIM || ldx < K || ldy < N || !group_ok(group) ||
         !type_ok(x_type) || !type_ok(y_type) || (epilogue != 0 && epilogue != 1) || ((uintptr_t)d_codes & 15) ||
         ((uintptr_t)d_scales & 1) || ((uintptr_t)d_X & (x_type == NERF_TYPE_BF16 ? 1 : 3)) ||
         ((uintptr_t)d_Y & (y_type == NERF_TYPE_BF16 ? 1 : 3)) || ((uintptr_t)d_workspace & 15))

@@ -167,6 +167,21 @@ def test_product_keeps_the_precision_of_fp32(gpu, m):
 
 
 @pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("m", [1, 2, 3, 20])
+def test_product_of_subnormal_inputs(gpu, m, bf16):
+    """X down to the smallest fp32 numbers against weights that are as large: no part of an input is taken for zero.  What
+    is below 2^-126 is exact as an input and in products, so the bound is check's, as for other inputs."""
+    n, k = 20, 200
+    rng = np.random.default_rng(m)
+    codes, scales = ref.quantize_w4((weights(n, k, 4) * np.float32(1e30)).astype(np.float32), 32)
+    w = ref.dequantize_w4(codes, scales, k, 32)
+    x = (rng.normal(size=(m, k)) * 10.0 ** rng.uniform(-42, -33, (m, k))).astype(np.float32)
+    held = ref.bf16(x) if bf16 else x
+    got = run(held, codes, scales, 32, n, k, bf16, False, 0)
+    check(got, (ref.from_bf16(held) if bf16 else x).astype(np.float64), w, False, 0)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
 @pytest.mark.parametrize("m", [1, 2, 6, 33])
 def test_values_that_are_not_finite(gpu, m, bf16):
     """an infinity or NaN in a row of X reaches that row of Y alone, as the formula has it; a NaN scale its own row of W"""
@@ -201,6 +216,97 @@ def test_same_bits_twice(gpu, m):
     x = rng.normal(size=(m, 5000)).astype(np.float32)
     a, b = (run(x, codes, scales, 64, 300, 5000, False, False, 0) for _ in range(2))
     assert np.array_equal(a, b)
+
+
+def test_more_rows_than_a_launch_takes(gpu):
+    m, n, k = 65535 * 64 + 70, 3, 5
+    rng = np.random.default_rng(8)
+    codes, scales = ref.quantize_w4(weights(n, k, 9), 32)
+    x = rng.normal(size=(m, k)).astype(np.float32)
+    check(run(x, codes, scales, 32, n, k, False, False, 0), x.astype(np.float64), ref.dequantize_w4(codes, scales, k, 32), False, 0)
+
+
+@pytest.mark.parametrize("m", [1, 24])
+def test_graphs_and_streams(gpu, m):
+    """quantize, a product (of 24 rows: with parts and their join) and dequantize in one graph on another stream than the
+    default, replayed with other weights in place each time, other work in between"""
+    import ctypes as C
+    torch = pytest.importorskip("torch")
+    from nerf_amd._lib import lib
+    n, k, group = 300, 2050, 64
+    size = lib.nerf_gemm_w4_workspace(m, n, k)
+    assert (size > 0) == (m == 24)
+    new = lambda shape, t: torch.empty(shape, dtype=t, device="cuda")
+    src, x = new((n, k), torch.float32), torch.randn(m, k, device="cuda")
+
+    def buffers():
+        return (new((n, lib.nerf_w4_row_bytes(k)), torch.uint8), new((n, -(-k // group)), torch.int16), new((m, n), torch.float32),
+                new((n, k), torch.float32), new(size + 16, torch.uint8))
+
+    def calls(codes, scales, y, back, ws):
+        return (lib.nerf_quantize_w4(src.data_ptr(), k, n, k, group, codes.data_ptr(), scales.data_ptr()),
+                lib.nerf_gemm_w4(x.data_ptr(), 0, k, codes.data_ptr(), scales.data_ptr(), group, y.data_ptr(), 0, n, m, n, k, 0,
+                                 ws.data_ptr(), size),
+                lib.nerf_dequantize_w4(codes.data_ptr(), scales.data_ptr(), n, k, group, back.data_ptr(), k))
+
+    mine, other = buffers(), buffers()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    src.normal_()
+    torch.cuda.synchronize()
+    try:
+        with torch.cuda.graph(graph, stream=side):
+            lib.nerf_set_stream(C.c_void_p(side.cuda_stream))
+            assert calls(*mine) == (0, 0, 0)
+    finally:
+        lib.nerf_set_stream(None)
+    for _ in range(3):
+        src.normal_()
+        for b in mine:
+            b.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert calls(*other) == (0, 0, 0)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(mine[:4], other[:4])) and mine[2].abs().max() > 0
+
+
+def test_trained_with_8_bit_states_and_answered_in_4_bits(gpu):
+    """the operators together: gradients of the trainer, their norm, a clipped 8-bit step on its weights, those weights in
+    4 bits, and their products with one point and with a few"""
+    from conftest import make_scene
+    from nerf_amd._lib import lib
+    from nerf_amd.api import AdamW, DeviceArray, HostDataset, Trainer, make_camera, trainer_config
+    cams, images = make_scene(3, 32, 24)
+    dds = HostDataset([make_camera(*c) for c in cams], images).upload()
+    tr = Trainer(trainer_config(rays_per_batch=8))
+    tr.init_weights(seed=2)
+    tensors, shapes = [], []
+    for o, (rows, cols) in tr.param_slices():
+        size, blocks = rows * cols, lib.nerf_adamw_state_blocks(rows * cols)
+        states = {s: DeviceArray.zeros(c, np.uint8) for s, c in (("m", size), ("v", size), ("m_exp", blocks), ("v_exp", blocks))}
+        tensors.append(dict(w=tr.params_ptr() + 4 * o, g=tr.grads_ptr() + 4 * o, n=size, **states))
+        shapes.append((o, rows, cols))
+    plan, norm = AdamW(tensors, state_bits=8), DeviceArray.zeros(1)
+    rng = np.random.default_rng(0)
+    before = tr.get_params()
+    for step in range(1, 3):
+        idx = np.stack([rng.integers(0, 3, 8), rng.integers(0, 32, 8), rng.integers(0, 24, 8)], axis=1).astype(np.int32)
+        tr.forward_backward(dds, DeviceArray.from_numpy(idx))
+        plan.grad_norm(norm, float(tr.N))
+        plan.step(step, 1e-3, float(tr.N), norm, 1e-3, seed=3)
+    params = tr.get_params()
+    assert (params != before).mean() > 0.9
+    for o, rows, cols in shapes:
+        w = params[o:o + rows * cols].reshape(rows, cols)
+        codes, scales = ref.quantize_w4(w, 64)
+        d_c, d_s = DeviceArray(codes.shape, np.uint8), DeviceArray(scales.shape, np.uint16)
+        assert lib.nerf_quantize_w4(tr.params_ptr() + 4 * o, cols, rows, cols, 64, d_c.ptr, d_s.ptr) == 0
+        assert np.array_equal(d_c.numpy(), codes) and np.array_equal(d_s.numpy(), scales)
+        for m in (1, 5):
+            x = rng.normal(size=(m, cols)).astype(np.float32)
+            check(run(x, d_c.numpy(), d_s.numpy(), 64, rows, cols, False, False, 0), x.astype(np.float64),
+                  ref.dequantize_w4(codes, scales, cols, 64), False, 0)
 
 
 def test_a_model_in_4_bits(gpu):

@@ -30,7 +30,7 @@ def test_ties_go_to_the_even_code():
 
 GOOD_Q = dict(src=0x1000, ld=100, rows=4, cols=100, group=32, codes=0x2000, scales=0x3000)
 BAD_Q = [dict(src=None), dict(codes=None), dict(scales=None), dict(rows=0), dict(cols=-1), dict(ld=99), dict(group=16), dict(group=0),
-         dict(src=0x1002), dict(codes=0x2008), dict(scales=0x3001)]
+         dict(src=0x1002), dict(codes=0x2008), dict(scales=0x3001), dict(cols=(1 << 30) + 1, ld=1 << 31)]
 
 
 @pytest.mark.parametrize("bad", BAD_Q, ids=str)
@@ -45,7 +45,7 @@ GOOD_P = dict(x=0x1000, xt=0, ldx=100, codes=0x2000, scales=0x3000, group=64, y=
               wb=1 << 30)
 BAD_P = [dict(x=None), dict(codes=None), dict(scales=None), dict(y=None), dict(m=0), dict(n=0), dict(k=0), dict(ldx=99), dict(ldy=7),
          dict(group=48), dict(xt=2), dict(yt=-1), dict(epi=2), dict(x=0x1002), dict(x=0x1001, xt=1), dict(codes=0x2004),
-         dict(scales=0x3001), dict(y=0x4001), dict(y=0x4002, yt=0), dict(ws=0x8004)]
+         dict(scales=0x3001), dict(y=0x4001), dict(y=0x4002, yt=0), dict(ws=0x8004), dict(k=(1 << 30) + 1, ldx=1 << 31), dict(n=(1 << 30) + 1, ldy=1 << 31)]
 
 
 def _product(lib, p):
