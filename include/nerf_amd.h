@@ -152,8 +152,9 @@ size_t nerf_adamw_state_blocks(size_t n);
 /* A plan over `count` tensors on the current device.  state_bits: 32, 8, or 0 for a plan that only takes norms (it
  * reads g, grad_type and n of each tensor).  The list is copied; its pointers (device memory, aligned to their
  * elements) must stay valid while the plan is used, and their contents are the caller's.  Zeroed states are the
- * start.  Returns 1 for a bad argument: among them a buffer that a step writes and that overlaps another one of
- * the list, and a pointer to pageable host memory or another GPU. */
+ * start.  A list has up to 2^22 - 1 runs of 4096 elements (a tensor's last run may be shorter).  Returns 1 for a bad
+ * argument: among them a buffer that a step writes and that overlaps another one of the list, a pointer to pageable host
+ * memory or another GPU, a buffer longer than its allocation, and a stream that is being captured. */
 int nerf_adamw_create(const NerfAdamwTensor* tensors, int count, int state_bits, float beta1, float beta2, float eps,
                       NerfAdamw** out);
 /* waits for the device's work and frees the plan's own tables */
@@ -199,7 +200,8 @@ int nerf_dequantize_w4(const unsigned char* d_codes, const unsigned short* d_sca
  * apart, epilogue 0: act is nothing, 1: swish.  Products are exact, sums are in fp32 and Y is rounded once.  Made for
  * few rows (one to some dozens); for hundreds, dequantize once and use nerf_gemm_f32 or nerf_gemm_bf16_nt.  Needs
  * d_codes 16-byte aligned.  d_workspace: nerf_gemm_w4_workspace bytes, 16-byte aligned (may be NULL where that is 0);
- * calls that overlap in time need one each. */
+ * calls that overlap in time need one each, replays of captured ones included.  Y overlaps neither an input nor the
+ * workspace. */
 size_t nerf_gemm_w4_workspace(int M, int N, int K);
 int nerf_gemm_w4(const void* d_X, int x_type, long ldx, const unsigned char* d_codes, const unsigned short* d_scales,
                  int group, void* d_Y, int y_type, long ldy, int M, int N, int K, int epilogue, void* d_workspace,

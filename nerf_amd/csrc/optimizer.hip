@@ -534,6 +534,13 @@ extern "C" {
 
 size_t nerf_adamw_state_blocks(size_t n) { return n / BLOCK + (n % BLOCK != 0); }
 
+// NERF_OK, or NERF_ERR_ARG while the library's stream is being captured into a graph
+static int not_capturing() {
+    hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(stream(), &capturing) != hipSuccess) return NERF_ERR_HIP;
+    return capturing == hipStreamCaptureStatusNone ? NERF_OK : NERF_ERR_ARG;
+}
+
 static int build_plan(const NerfAdamwTensor* tensors, int count, int state_bits, NerfAdamw* plan) {
     size_t pieces = 0;
     for (int k = 0; k < count; k++) {
@@ -583,6 +590,8 @@ static int build_plan(const NerfAdamwTensor* tensors, int count, int state_bits,
         first += s.n;
     }
     plan->chunks = (unsigned)pieces;
+    const int rc = not_capturing();  // the wait below would end the capture
+    if (rc != NERF_OK) return rc;
     if (hipMalloc(&plan->memory, image.size()) != hipSuccess) return NERF_ERR_HIP;
     plan->d_partial = (unsigned long long*)plan->memory;
     plan->d_ticket = (unsigned*)((char*)plan->memory + NORM_BLOCKS * sizeof(unsigned long long));
@@ -639,10 +648,8 @@ int nerf_adamw_step(NerfAdamw* plan, int step, float learning_rate, float grad_d
     if (!plan || !plan->state_bits || step < 1 || !finite_not_negative(learning_rate) || !(grad_div > 0.0f && grad_div < INFINITY) ||
         (d_norm && !(max_norm > 0.0f && max_norm < INFINITY)) || !plan_usable(plan))
         return NERF_ERR_ARG;
-    // a graph would repeat this step number and learning rate for ever
-    hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(stream(), &capturing) != hipSuccess) return NERF_ERR_HIP;
-    if (capturing != hipStreamCaptureStatusNone) return NERF_ERR_ARG;
+    const int rc = not_capturing();  // a graph would repeat this step number and learning rate for ever
+    if (rc != NERF_OK) return rc;
     if (!plan->chunks) return NERF_OK;
     StepArgs a = {};
     a.chunks = plan->d_chunks;

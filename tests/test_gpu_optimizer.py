@@ -370,6 +370,31 @@ def test_graphs_and_streams(gpu):
     assert np.array_equal(case.aw.read()[0], other.aw.read()[0]) and np.array_equal(case.am.read()[0], other.am.read()[0])
 
 
+def test_no_plan_is_made_while_a_stream_is_captured(gpu):
+    """refused before anything that would end the capture: the norm captured beside it replays"""
+    torch = pytest.importorskip("torch")
+    from nerf_amd._lib import lib
+    from nerf_amd.api import AdamW
+    case, norm, want = Case([5000], 32, 3), torch.zeros(1, device="cuda"), torch.zeros(1, device="cuda")
+    case.plan.grad_norm(want.data_ptr())
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    try:
+        with torch.cuda.graph(graph, stream=side, capture_error_mode="relaxed"):
+            lib.nerf_set_stream(C.c_void_p(side.cuda_stream))
+            with pytest.raises(Exception, match="nerf_adamw_create"):
+                AdamW([dict(g=norm.data_ptr(), n=1)], state_bits=0)
+            case.plan.grad_norm(norm.data_ptr())
+    finally:
+        lib.nerf_set_stream(None)
+    for _ in range(2):
+        norm.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert norm.item() == want.item() != 0.0
+
+
 def test_training_step_with_8_bit_states(gpu):
     """forward and backward of the trainer, the norm, and the clipped 8-bit step on the trainer's own arenas: three
     steps, each against the formula on the gradients and states the device held before it"""
