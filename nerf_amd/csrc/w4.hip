@@ -441,52 +441,48 @@ __device__ __forceinline__ u32x4 transpose4(u32x4 d) {
     return u32x4{c[0], c[1], e[0], e[1]};
 }
 
-// A chunk of one of a lane's rows of W as it lies in memory: its codes, and the scales of its groups.  In the last chunk of
-// a row that is no multiple of 128 long, a unit past the row's end is the last one again (X is zero there), and the
-// scales are those of the row's last groups: `past` bits too far up, above which there is zero for the groups that are
-// not there.  Nothing is done to what is loaded before it is used, or the load would be waited for.
-template <int GROUP>
-struct Chunk4 {
-    static constexpr int GROUPS = 128 / GROUP;
-    u32x4 codes;
-    unsigned scales[GROUP == 32 ? 2 : 1];
+// Up to eight consecutive scales of a row of W, from `first` on, as they lie in memory; the row has `groups`.  At the row's
+// end they are its last COUNT ones, and the shift is left to put(): nothing is done to what is loaded before it is used, or
+// the load would be waited for.  Groups past the end have the scale zero.
+template <int COUNT>
+struct Scales {
+    unsigned v[COUNT <= 2 ? 1 : COUNT / 2];
 
-    // unit: of the lane, in a row of `units`; first: the chunk's first group, in a row of `groups`
-    __device__ __forceinline__ void load(const unsigned char* codes_row, const unsigned short* scales_row, int unit, int units, int first,
-                                         int groups) {
-        codes = *reinterpret_cast<const u32x4*>(codes_row + (long)min(unit, units - 1) * 16);
-        if (groups >= GROUPS) {
-            const unsigned short* p = scales_row + min(first, groups - GROUPS);
-            if constexpr (GROUP == 32) {
-                const u32x2u s = *reinterpret_cast<const u32x2u*>(p);
-                scales[0] = s[0];
-                scales[1] = s[1];
-            } else if constexpr (GROUP == 64) {
-                scales[0] = *reinterpret_cast<const u32u*>(p);
+    __device__ __forceinline__ void load(const unsigned short* row, int first, int groups) {
+        if (groups >= COUNT) {
+            const unsigned short* p = row + min(first, groups - COUNT);
+            if constexpr (COUNT == 8) {
+                const u32x4u2 x = *reinterpret_cast<const u32x4u2*>(p);
+#pragma unroll
+                for (int k = 0; k < 4; k++) v[k] = x[k];
+            } else if constexpr (COUNT == 4) {
+                const u32x2u x = *reinterpret_cast<const u32x2u*>(p);
+                v[0] = x[0];
+                v[1] = x[1];
             } else {
-                scales[0] = *p;
+                v[0] = *reinterpret_cast<const u32u*>(p);
             }
-        } else {  // a row of one chunk with fewer groups
-            scales[0] = scales_row[0] | (groups > 1 ? (unsigned)scales_row[1] << 16 : 0u);
-            if constexpr (GROUP == 32) scales[1] = groups > 2 ? scales_row[2] : 0u;
+        } else {
+#pragma unroll
+            for (int k = 0; k < COUNT / 2; k++)
+                v[k] = (2 * k < groups ? row[2 * k] : 0u) | (2 * k + 1 < groups ? (unsigned)row[2 * k + 1] << 16 : 0u);
         }
     }
-    // the scales of the chunk's groups
-    __device__ __forceinline__ void take(int first, int groups, float* s) const {
-        const int past = max(0, first - (groups - GROUPS)) * (groups >= GROUPS ? 16 : 0);
-        if constexpr (GROUP == 32) {
-            const unsigned long long all = ((unsigned long long)scales[1] << 32 | scales[0]) >> past;
-            const unsigned lo = (unsigned)all, hi = (unsigned)(all >> 32);
-            s[0] = __builtin_bit_cast(float, lo << 16);
-            s[1] = __builtin_bit_cast(float, lo & 0xFFFF0000u);
-            s[2] = __builtin_bit_cast(float, hi << 16);
-            s[3] = __builtin_bit_cast(float, hi & 0xFFFF0000u);
-        } else if constexpr (GROUP == 64) {
-            const unsigned all = scales[0] >> past;
-            s[0] = __builtin_bit_cast(float, all << 16);
-            s[1] = __builtin_bit_cast(float, all & 0xFFFF0000u);
-        } else {
-            s[0] = __builtin_bit_cast(float, scales[0] << 16);
+    __device__ __forceinline__ void put(char* at, int first, int groups) const {
+        if (first + COUNT <= max(groups, COUNT)) {
+            if constexpr (COUNT == 8) *reinterpret_cast<u32x4*>(at) = u32x4{v[0], v[1], v[2], v[3]};
+            else
+#pragma unroll
+                for (int k = 0; k < COUNT / 2; k++) reinterpret_cast<unsigned*>(at)[k] = v[k];
+            return;
+        }
+        const int past = first - max(0, groups - COUNT);  // places too far up
+#pragma unroll
+        for (int k = 0; k < COUNT; k++) {
+            const unsigned short x = (unsigned short)(v[k / 2] >> (16 * (k & 1)));
+            unsigned short* to = reinterpret_cast<unsigned short*>(at);
+            if (k >= past) to[k - past] = x;
+            if (COUNT - 1 - k < past) to[k] = 0;
         }
     }
 };
@@ -494,19 +490,25 @@ struct Chunk4 {
 struct GemmShape {
     int log_kw;        // 2^log_kw wavefronts split the contraction: 1, 2, 4 or 8
     int split_chunks;  // chunks of one part of the contraction (gridDim.z parts), a multiple of a slice
+    int scales_at;     // bytes of LDS before the scales
     float* partial;    // [parts][M][N], or null: one part, stored to Y
 };
 
 constexpr int CUS = 256;
 constexpr int DEPTH = 2;  // chunks of W on their way to a wavefront
 
-// chunks of a slice: with this many, a slice of R MT rows is four pieces of eight columns for each thread
-constexpr int slice_chunks(int r, int mt) { return 128 / (r * mt); }
+// chunks of a slice: with this many, a slice of R MT rows is four pieces of eight columns for each thread, or two of four rows
+constexpr int slice_chunks(int r, int mt) { return r == 4 ? 16 : 8 / mt; }
+// scales of a row in a slice; a thread loads up to eight of them at once; bytes from row to row in LDS
+constexpr int slice_scales(int r, int mt, int group) { return slice_chunks(r, mt) * (128 / group); }
+constexpr int scales_pitch(int r, int mt, int group) { return slice_scales(r, mt, group) * 2 + 16; }
 
 template <int R, int MT, int NT, bool XBF, int GROUP>
 __global__ __launch_bounds__(64 * WAVES) void gemm_w4_kernel(const W4Args a, const GemmShape g) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    constexpr int PARTS = XBF ? 1 : 3, STEPS = GROUP / 32, SLICE = slice_chunks(R, MT);
+    constexpr int PARTS = XBF ? 1 : 3, STEPS = GROUP / 32, SLICE = slice_chunks(R, MT), PIECES = R * MT * SLICE / 32;
+    constexpr int SCALES = slice_scales(R, MT, GROUP), COUNT = SCALES < 8 ? SCALES : 8, RUNS = SCALES / COUNT, PITCH = scales_pitch(R, MT, GROUP);
+    constexpr int SCALE_TURNS = (16 * NT * WAVES * RUNS + 64 * WAVES - 1) / (64 * WAVES);
     // LDS: [step of 32 columns][part][tile of R rows][unit of 8 columns][row], 16 bytes each: a wavefront reads an operand as
     // one run; the steps are 16 bytes further apart, so that a run of a row's pieces is written to different banks
     constexpr int TILE_BYTES = R * 64, PART_BYTES = MT * TILE_BYTES, STEP_BYTES = PARTS * PART_BYTES + 16;
@@ -520,12 +522,10 @@ __global__ __launch_bounds__(64 * WAVES) void gemm_w4_kernel(const W4Args a, con
     const int chunks = (a.K + 127) / 128, units = (a.K + 31) / 32;
     const int first = blockIdx.z * g.split_chunks, end = min(chunks, first + g.split_chunks);
     const unsigned char* wrow[NT];
-    const unsigned short* srow[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) {  // rows past the end repeat the last one; what they give is not stored
         const long n = min(n0 + t * 16 + ln, (long)a.N - 1);
         wrow[t] = a.codes + n * a.row_bytes;
-        srow[t] = a.scales + n * a.groups;
     }
     // A wavefront's turns: SLICE / kw in each slice but the last, which has what is left.  Within a slice they begin at
     // a place that differs from workgroup to workgroup.
@@ -539,10 +539,10 @@ __global__ __launch_bounds__(64 * WAVES) void gemm_w4_kernel(const W4Args a, con
         if (i >= count) i -= count;
         return first + slice * SLICE + wk + (i << g.log_kw);
     };
-    auto load = [&](Chunk4<GROUP>* w, int turn) {
+    auto load = [&](u32x4* w, int turn) {
         const int c = chunk_of(min(turn, turns_all - 1));  // past the end: the last one again
 #pragma unroll
-        for (int t = 0; t < NT; t++) w[t].load(wrow[t], srow[t], c * 4 + lj, units, c * (128 / GROUP), a.groups);
+        for (int t = 0; t < NT; t++) w[t] = *reinterpret_cast<const u32x4*>(wrow[t] + (long)min(c * 4 + lj, units - 1) * 16);
     };
     f32x4 acc[MT][NT];
 #pragma unroll
@@ -550,13 +550,13 @@ __global__ __launch_bounds__(64 * WAVES) void gemm_w4_kernel(const W4Args a, con
 #pragma unroll
         for (int t = 0; t < NT; t++) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    // A thread's pieces of a slice: SLICE * 16 pieces in a row, R MT SLICE * 16 = 4 * 512 of them.  A piece that holds the
+    // A thread's pieces of a slice: SLICE * 16 pieces in a row, R MT SLICE * 16 = PIECES * 512 of them.  A piece that holds the
     // row's last columns and others past them is put together by itself.
-    Piece<XBF> piece[4];
+    Piece<XBF> piece[PIECES];
     auto at_piece = [&](int r, int p) { return lds + (p / 4) * STEP_BYTES + (r / R) * TILE_BYTES + ((p % 4) * R + r % R) * 16; };
     auto load_x = [&](int base) {
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < PIECES; k++) {
             const int q = threadIdx.x + k * 64 * WAVES, r = q / (SLICE * 16), col = base * 128 + q % (SLICE * 16) * 8;
             piece[k].zero();
             if (r < rows && col + 8 <= a.K) piece[k].load((const char*)a.X + (m0 + r) * a.ldx * (XBF ? 2 : 4), col);
@@ -565,7 +565,7 @@ __global__ __launch_bounds__(64 * WAVES) void gemm_w4_kernel(const W4Args a, con
     auto stage_x = [&](int base) {
         const int width = min(SLICE, end - base) * 16;  // pieces of a row that are looked at
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < PIECES; k++) {
             const int q = threadIdx.x + k * 64 * WAVES, r = q / (SLICE * 16), p = q % (SLICE * 16), col = base * 128 + p * 8;
             if (r < rows && p < width && (col + 8 <= a.K || col >= a.K)) {
                 u32x4 o[PARTS];
@@ -595,21 +595,59 @@ __global__ __launch_bounds__(64 * WAVES) void gemm_w4_kernel(const W4Args a, con
     // rows past the end are read as what LDS holds there, or as the last row where R < 16: their sums are not stored
     const char* xlane = lds + (lj * R + min(ln, R - 1)) * 16;
 
-    Chunk4<GROUP> w[DEPTH][NT];
+    // the scales of the slice, of all rows of W of the workgroup: read in runs along a row, once for the wavefronts that
+    // split the contraction, and one slice ahead like X
+    Scales<COUNT> scales[SCALE_TURNS];
+    auto scales_of = [&](int k, int& row, int& run) {
+        const int q = threadIdx.x + k * 64 * WAVES;
+        row = q / RUNS, run = q % RUNS;
+        return row < columns * 16 * NT;
+    };
+    auto load_scales = [&](int base) {
+#pragma unroll
+        for (int k = 0; k < SCALE_TURNS; k++) {
+            int row, run;
+            if (scales_of(k, row, run)) {
+                const long n = min((long)blockIdx.x * (columns * 16 * NT) + row, (long)a.N - 1);
+                scales[k].load(a.scales + n * a.groups, base * (128 / GROUP) + run * COUNT, a.groups);
+            }
+        }
+    };
+    auto stage_scales = [&](int base) {
+#pragma unroll
+        for (int k = 0; k < SCALE_TURNS; k++) {
+            int row, run;
+            if (scales_of(k, row, run)) scales[k].put(lds + g.scales_at + row * PITCH + run * COUNT * 2, base * (128 / GROUP) + run * COUNT, a.groups);
+        }
+    };
+    const char* slane = lds + g.scales_at + (wn * 16 * NT + ln) * PITCH;
+
+    u32x4 w[DEPTH][NT];
+    load_scales(first);
     load_x(first);  // before W: loads come back in their order, and X is waited for first
     if (turns_all) {
 #pragma unroll
         for (int d = 0; d < DEPTH; d++) load(w[d], d);
     }
-    auto chunk = [&](const Chunk4<GROUP>* w, int turn, int base) {
-        const int c = chunk_of(turn);
-        const char* xs = xlane + (c - base) * (4 * STEP_BYTES);
+    auto chunk = [&](const u32x4* w, int turn, int base) {
+        const int at = chunk_of(turn) - base;
+        const char* xs = xlane + at * (4 * STEP_BYTES);
         u32x4 codes[NT];
         float scales[NT][128 / GROUP];
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            codes[t] = transpose4(w[t].codes);
-            w[t].take(c * (128 / GROUP), a.groups, scales[t]);
+            codes[t] = transpose4(w[t]);
+            const char* from = slane + t * 16 * PITCH + at * (256 / GROUP);
+            if constexpr (GROUP == 128) {
+                scales[t][0] = bf16_to_f32(*reinterpret_cast<const unsigned short*>(from));
+            } else {
+#pragma unroll
+                for (int k = 0; k < 64 / GROUP; k++) {
+                    const unsigned two = reinterpret_cast<const unsigned*>(from)[k];
+                    scales[t][2 * k] = __builtin_bit_cast(float, two << 16);
+                    scales[t][2 * k + 1] = __builtin_bit_cast(float, two & 0xFFFF0000u);
+                }
+            }
         }
         f32x4 part[MT][NT];
 #pragma unroll
@@ -641,7 +679,10 @@ __global__ __launch_bounds__(64 * WAVES) void gemm_w4_kernel(const W4Args a, con
     int turn = 0;
     for (int base = first - SLICE; base < end; base += SLICE) {  // the first time round there is no slice yet
         const bool more = base + SLICE < end;
-        if (more && base >= first) load_x(base + SLICE);
+        if (more && base >= first) {
+            load_scales(base + SLICE);
+            load_x(base + SLICE);
+        }
         if (base >= first) {
             const int stop = min(turns_all, turn + (1 << log_turns));
             // a whole slice has a multiple of DEPTH turns
@@ -656,6 +697,7 @@ __global__ __launch_bounds__(64 * WAVES) void gemm_w4_kernel(const W4Args a, con
             __syncthreads();
         }
         if (more) {
+            stage_scales(base + SLICE);
             stage_x(base + SLICE);
             __syncthreads();
         }
@@ -756,9 +798,9 @@ template <int R, int MT, int NT, bool XBF, int GROUP>
 hipError_t launch_gemm(const W4Args& a, const GemmPlan& p, float* partial) {
     constexpr int PARTS = XBF ? 1 : 3;
     const size_t x_bytes = (size_t)std::min(slice_chunks(R, MT), p.split_chunks) * 4 * (PARTS * MT * R * 64 + 16);
-    const size_t bytes = std::max(x_bytes, (size_t)WAVES * NT * 64 * 16);
     const long columns = 16L * NT * (WAVES >> p.log_kw);
-    const GemmShape shape = {p.log_kw, p.split_chunks, p.parts > 1 ? partial : nullptr};
+    const size_t bytes = std::max(x_bytes + (size_t)columns * scales_pitch(R, MT, GROUP), (size_t)WAVES * NT * 64 * 16);
+    const GemmShape shape = {p.log_kw, p.split_chunks, (int)x_bytes, p.parts > 1 ? partial : nullptr};
     constexpr long MOST = 65535L * R * MT;  // rows of a launch: gridDim.y has 16 bits
     for (long m = 0; m < a.M; m += MOST) {
         W4Args some = a;
