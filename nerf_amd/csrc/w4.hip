@@ -358,11 +358,11 @@ __global__ __launch_bounds__(64 * WAVES) void gemv_w4_kernel(const W4Args a, con
 // (16 x 16 x 32), so that a step's 32 columns lie in one group and the sum over a group takes one scale.  Columns of
 // workgroups start at different chunks of a slice: rows of W are often a power of two apart, and workgroups that walk
 // them in step would all ask the same few memory channels.
-//   Times (groups of 64): 24 x 4100 x 4090 16.2 us (bf16 12.6), of which W's bytes are 1.4 us, two launches 5, and the rest a
-// chain that is too short to overlap: X arrives and is split, W arrives, matrix instructions, sums written and read again.
-// 16 x 16384 x 8192 29.3 us = 2.4 TB/s of W (every workgroup of 256 columns reads as many bytes of X from the L2 as half its
-// own of W, and each wavefront reads all of them again from LDS); 64 x 16384 x 8192 in bf16 38.7 us = 443 TFLOP/s.  Eight
-// chunks of W ahead instead of DEPTH, or four wavefronts instead of eight, measured the same to 15 % slower.
+//   Times (groups of 64): 16 x 16384 x 8192 24.9 us = 2.9 TB/s of W; left out by turns, X costs 7 us of it, matrix instructions
+// and conversions 4.5, and W, two launches and the join the rest.  24 x 4100 x 4090 14.5 us: X 4, the second
+// launch and the join 4.5, the rest a chain that is too short to overlap.  64 x 16384 x 8192 60 us, in bf16 35 = 490 TFLOP/s.
+// Scales that each wavefront loads for itself, chunk by chunk (16 lines for 64 bytes of each row), had cost 5 us of
+// 8 x 16384 x 8192 in bf16 (18.9 us); sixteen wavefronts to a workgroup, or a whole slice of W ahead, gained nothing.
 // eight codes as eight bf16
 __device__ __forceinline__ bf16x8 values8_bf16(unsigned c) {
     const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, 1.0f, 1);
@@ -497,17 +497,20 @@ struct GemmShape {
 constexpr int CUS = 256;
 constexpr int DEPTH = 2;  // chunks of W on their way to a wavefront
 
-// chunks of a slice: with this many, a slice of R MT rows is four pieces of eight columns for each thread, or two of four rows
-constexpr int slice_chunks(int r, int mt) { return r == 4 ? 16 : 8 / mt; }
-// scales of a row in a slice; a thread loads up to eight of them at once; bytes from row to row in LDS
-constexpr int slice_scales(int r, int mt, int group) { return slice_chunks(r, mt) * (128 / group); }
-constexpr int scales_pitch(int r, int mt, int group) { return slice_scales(r, mt, group) * 2 + 16; }
+// Chunks of a slice, of X in R MT rows and of the scales: few enough that X in fp32 leaves room in LDS and that parts of the
+// contraction come out even (24 x 4100 x 4090: 14.4 us with 2, 15.6 with 4), and enough to cover the time of a read while
+// a slice is worked on (16 x 16384 x 8192: 24.5 us with 8, 25.6 with 4; 32 x 16384 x 8192 in bf16 with half of the parts:
+// 26 with 4, 33 with 2).
+constexpr int slice_chunks(int r, int mt, bool x_bf16) { return r == 4 ? 16 : mt == 1 ? 8 : x_bf16 ? 4 : 2; }
+// scales of a row in a slice; bytes from row to row in LDS
+constexpr int slice_scales(int slice, int group) { return slice * (128 / group); }
+constexpr int scales_pitch(int slice, int group) { return slice_scales(slice, group) * 2 + 16; }
 
 template <int R, int MT, int NT, bool XBF, int GROUP>
 __global__ __launch_bounds__(64 * WAVES) void gemm_w4_kernel(const W4Args a, const GemmShape g) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    constexpr int PARTS = XBF ? 1 : 3, STEPS = GROUP / 32, SLICE = slice_chunks(R, MT), PIECES = R * MT * SLICE / 32;
-    constexpr int SCALES = slice_scales(R, MT, GROUP), COUNT = SCALES < 8 ? SCALES : 8, RUNS = SCALES / COUNT, PITCH = scales_pitch(R, MT, GROUP);
+    constexpr int PARTS = XBF ? 1 : 3, STEPS = GROUP / 32, SLICE = slice_chunks(R, MT, XBF), PIECES = R * MT * SLICE / 32;
+    constexpr int SCALES = slice_scales(SLICE, GROUP), COUNT = SCALES < 8 ? SCALES : 8, RUNS = SCALES / COUNT, PITCH = scales_pitch(SLICE, GROUP);
     constexpr int SCALE_TURNS = (16 * NT * WAVES * RUNS + 64 * WAVES - 1) / (64 * WAVES);
     // LDS: [step of 32 columns][part][tile of R rows][unit of 8 columns][row], 16 bytes each: a wavefront reads an operand as
     // one run; the steps are 16 bytes further apart, so that a run of a row's pieces is written to different banks
@@ -759,47 +762,65 @@ __global__ __launch_bounds__(256) void join_w4_kernel(const W4Args a, const floa
         if (r < columns) store_y(a, m * a.ldy + n + r, y[r]);
 }
 
+struct Costs {
+    float x, weight, product, read, slice, join, part, value;
+};
+constexpr Costs F32_COSTS = {1.35e-4f, 2.4e-5f, 1.3e-5f, 0.0f, 0.36f, 4.0f, 0.09f, 3.1e-6f};
+constexpr Costs BF16_COSTS = {1.33e-5f, 7.9e-6f, 7.6e-6f, 4.4e-6f, 0.36f, 2.0f, 0.07f, 1.4e-6f};
+
 struct GemmPlan {
     int r, mt, nt, log_kw, parts, split_chunks;
 };
 
-// Which wavefronts share what (times: groups of 64, X in fp32 unless it says bf16):
-//   Rows of X to a workgroup: all of them up to 64, so that W is read and converted once.
-//   Columns of a wavefront: 32 where there are many, since a tile of X read from LDS then serves two tiles of W: 16 x 16384
-// x 8192 takes 30.2 us with 32 and 33.9 with 16, 64 x 16384 x 8192 62.8 and 77.4 (bf16: 39.4 and 38.0).  But 16 where only
-// that gives every CU a workgroup of its own: 64 x 32768 x 1024 takes 25.2 us with 16 and 29.7 with 32.
-//   Wavefronts along the contraction, which cost nothing but a narrower workgroup, so that X is read more often.  Up to
-// four rows X is small, and they go up to a workgroup for each CU: 3 x 4096 x 4096 takes 6.4, 8.6 and 33 us with 8, 4 and 1.
-// Else they go up to 64 workgroups: 16 x 4096 x 4096 takes 10.9 us with 2 and four parts, 12.3 with 4 and three, 11.5 with 1
-// and eight.
-//   Parts of the contraction, each in workgroups of its own, fill the CUs then.  They are joined by a second kernel, about
-// 3 us, and a part has at least a slice of X: 16 x 256 x 16384 in bf16 takes 9.8 us with 16 parts, 11.2 with 32 or 8.
-GemmPlan plan_gemm(int M, int N, int K) {
-    GemmPlan p = {};
-    const int chunks = K / 128 + (K % 128 != 0);
-    p.r = M <= 4 ? 4 : 16;
-    p.mt = M <= 16 ? 1 : M <= 32 ? 2 : 4;
-    const int slice = slice_chunks(p.r, p.mt);
-    const long m_blocks = (M + p.r * p.mt - 1L) / (p.r * p.mt);
-    auto blocks = [&](int nt) {
-        const int columns = 16 * nt * (WAVES >> p.log_kw);
-        return ((long)N + columns - 1) / columns * m_blocks;
-    };
-    p.nt = N >= 8192 && (blocks(2) >= CUS || blocks(1) < CUS) ? 2 : 1;
-    while (blocks(p.nt) < (p.r == 4 ? CUS : CUS / 4) && (slice >> p.log_kw) > DEPTH && (chunks >> p.log_kw) > 1 && p.log_kw < 3) p.log_kw++;
-    p.parts = (int)std::max(1L, std::min(std::min(64L, (long)chunks / (8 / p.mt)), CUS / blocks(p.nt)));
-    p.split_chunks = (chunks + p.parts - 1) / p.parts;
-    if (p.parts > 1 && p.split_chunks > slice) p.split_chunks = (p.split_chunks + slice - 1) / slice * slice;
-    p.parts = (chunks + p.split_chunks - 1) / p.split_chunks;
-    return p;
+// The shape of a launch is the one whose estimated time is least (us on 256 CUs, a workgroup at a time on each): so much for
+// a value of X (brought in, split, put in LDS), for a weight (brought in and converted), for a weight and a tile of rows
+// (multiplied), for a tile of X read from LDS for 16 NT columns, for a slice, for the second kernel that joins parts, for a part,
+// and for a value of one (written and read).  The numbers are fitted to 2100 measured launches of 37 shapes (3 to 200
+// rows, 200 to 32768 columns, K from 500 to 16384) so that the shapes they find are the fastest ones measured: they
+// are within 11 % of those, and 24 x 4100 x 4090 in bf16 within 16 (12.9 us for 11.2).  What decides, with both sides measured:
+//   rows to a workgroup: 64 x 16384 x 8192 61 us with 64 and 70 with 16, but 64 x 512 x 512 12.3 and 5.1
+//   columns of a wavefront, 16 or 32: 16 x 16384 x 8192 30.4 and 25.4 us, but 4 x 512 x 512 4.3 and 5.1
+//   wavefronts along the contraction: 3 x 4096 x 4096 6.2, 7.6 and 29 us with 8, 4 and 1; 16 x 16384 x 8192 25.4 with 1, 28.5 with 2
+//   parts: 24 x 4100 x 4090 14.4 us with 6 (a join among them), 15.7 with 4; 64 x 4096 x 4096 in bf16 10.8 with 1, 12.5 with 3
+GemmPlan plan_gemm(int M, int N, int K, bool x_bf16) {
+    GemmPlan best = {};
+    const int chunks = K / 128 + (K % 128 != 0), r = M <= 4 ? 4 : 16;
+    const Costs& of = x_bf16 ? BF16_COSTS : F32_COSTS;
+    float least = INFINITY;
+    for (int mt = 1; mt == 1 || (mt <= 4 && 8 * mt < M); mt *= 2) {
+        const int slice = slice_chunks(r, mt, x_bf16);
+        const long m_blocks = (M + r * mt - 1L) / (r * mt);
+        for (int nt = 1; nt <= 2; nt++)
+            for (int log_kw = 0; log_kw <= 3 && slice >> log_kw >= DEPTH && chunks >> log_kw; log_kw++) {
+                const int columns = 16 * nt * (WAVES >> log_kw);
+                const long blocks = ((long)N + columns - 1) / columns * m_blocks;
+                // as many parts as there are CUs for, half or a quarter of them, and one
+                for (long want = std::min(std::min(64L, (long)chunks), std::max(1L, CUS / blocks)), turn = 0; turn < 4; turn++) {
+                    const int parts = turn == 3 ? 1 : (int)(want >> turn);
+                    if (parts < 1 || (parts == 1 && turn < 3)) continue;
+                    int split = (chunks + parts - 1) / parts;
+                    if (parts > 1 && split > slice) split = (split + slice - 1) / slice * slice;
+                    const int used = (chunks + split - 1) / split;
+                    const float depth = (float)std::min(split * 128L, (long)K), slices = (float)((split + slice - 1) / slice);
+                    const float work = depth * (of.x * std::min(M, r * mt) + columns * (of.weight + mt * (of.product + of.read / nt))) + of.slice * slices;
+                    float cost = (float)((blocks * used + CUS - 1) / CUS) * work;
+                    if (used > 1) cost += of.join + used * (of.part + of.value * M * N);
+                    if (cost < least) {
+                        least = cost;
+                        best = {r, mt, nt, log_kw, used, split};
+                    }
+                }
+            }
+    }
+    return best;
 }
 
 template <int R, int MT, int NT, bool XBF, int GROUP>
 hipError_t launch_gemm(const W4Args& a, const GemmPlan& p, float* partial) {
-    constexpr int PARTS = XBF ? 1 : 3;
-    const size_t x_bytes = (size_t)std::min(slice_chunks(R, MT), p.split_chunks) * 4 * (PARTS * MT * R * 64 + 16);
+    constexpr int PARTS = XBF ? 1 : 3, SLICE = slice_chunks(R, MT, XBF);
+    const size_t x_bytes = (size_t)std::min(SLICE, p.split_chunks) * 4 * (PARTS * MT * R * 64 + 16);
     const long columns = 16L * NT * (WAVES >> p.log_kw);
-    const size_t bytes = std::max(x_bytes + (size_t)columns * scales_pitch(R, MT, GROUP), (size_t)WAVES * NT * 64 * 16);
+    const size_t bytes = std::max(x_bytes + (size_t)columns * scales_pitch(SLICE, GROUP), (size_t)WAVES * NT * 64 * 16);
     const GemmShape shape = {p.log_kw, p.split_chunks, (int)x_bytes, p.parts > 1 ? partial : nullptr};
     constexpr long MOST = 65535L * R * MT;  // rows of a launch: gridDim.y has 16 bits
     for (long m = 0; m < a.M; m += MOST) {
@@ -850,6 +871,7 @@ hipError_t launch_gemv(const W4Args& a) {
     return hipGetLastError();
 }
 
+size_t plan_bytes(const GemmPlan& p, int M, int N) { return p.parts > 1 ? (size_t)p.parts * M * N * sizeof(float) : 0; }
 bool group_ok(int group) { return group == 32 || group == 64 || group == 128; }
 bool type_ok(int t) { return t == NERF_TYPE_F32 || t == NERF_TYPE_BF16; }
 int ceil_div(int a, int b) { return a / b + (a % b != 0); }
@@ -899,8 +921,7 @@ int nerf_dequantize_w4(const unsigned char* d_codes, const unsigned short* d_sca
 
 size_t nerf_gemm_w4_workspace(int M, int N, int K) {
     if (M <= 2 || N <= 0 || K <= 0) return 0;
-    const GemmPlan p = plan_gemm(M, N, K);
-    return p.parts > 1 ? (size_t)p.parts * M * N * sizeof(float) : 0;
+    return std::max(plan_bytes(plan_gemm(M, N, K, false), M, N), plan_bytes(plan_gemm(M, N, K, true), M, N));
 }
 
 int nerf_gemm_w4(const void* d_X, int x_type, long ldx, const unsigned char* d_codes, const unsigned short* d_scales,
@@ -911,7 +932,9 @@ int nerf_gemm_w4(const void* d_X, int x_type, long ldx, const unsigned char* d_c
         ((uintptr_t)d_scales & 1) || ((uintptr_t)d_X & (x_type == NERF_TYPE_BF16 ? 1 : 3)) ||
         ((uintptr_t)d_Y & (y_type == NERF_TYPE_BF16 ? 1 : 3)) || ((uintptr_t)d_workspace & 15))
         return NERF_ERR_ARG;
-    const size_t need = nerf_gemm_w4_workspace(M, N, K);
+    GemmPlan p = {};
+    if (M > 2) p = plan_gemm(M, N, K, x_type == NERF_TYPE_BF16);
+    const size_t need = plan_bytes(p, M, N);
     if (workspace_bytes < need || (need && !d_workspace)) return NERF_ERR_ARG;
     W4Args a = {};
     a.X = d_X; a.codes = d_codes; a.scales = d_scales; a.Y = d_Y;
@@ -919,7 +942,6 @@ int nerf_gemm_w4(const void* d_X, int x_type, long ldx, const unsigned char* d_c
     a.M = M; a.N = N; a.K = K; a.group = group; a.groups = ceil_div(K, group);
     a.x_bf16 = x_type == NERF_TYPE_BF16; a.y_bf16 = y_type == NERF_TYPE_BF16; a.epilogue = epilogue;
     ProfScope prof(K_GEMM_W4, 2.0 * M * N * K);
-    const GemmPlan p = plan_gemm(M, N, K);
     float* partial = (float*)d_workspace;
     hipError_t rc;
     if (M == 1) rc = launch_gemv<1>(a);
