@@ -34,9 +34,9 @@ struct SplitFrag {
     bf16x8 hi, lo;
 };
 
-// eight operand values -> their bf16 head and bf16 remainder.  Written on pairs so that each step is
+// eight operand values -> their bf16 head and bf16 remainder.  Written on pairs so that a conversion is
 // one packed instruction: v_cvt_pk_bf16_f32 (round to nearest even), shift / mask back to fp32,
-// v_pk_add_f32 for the exact remainder, v_cvt_pk_bf16_f32 again: 2.5 vector instructions per value.
+// v_sub_f32 for the exact remainder, v_cvt_pk_bf16_f32 again: 3 vector instructions per value.
 __device__ __forceinline__ SplitFrag split8(const float (&x)[8]) {
     u32x4 h, l;
 #pragma unroll

@@ -50,7 +50,8 @@ __device__ __forceinline__ long piece_of(unsigned id, unsigned per_row, int rows
 }
 
 // A thread takes eight consecutive columns of a row; the 4, 8 or 16 threads of a group are neighbours in a row of sixteen
-// lanes (a row of W has whole groups of threads).
+// lanes (a row of W has whole groups of threads).  Bound by memory: 8192 x 8192 57 us = 5.3 TB/s; two such pieces to a thread
+// 58, reads past the caches 60, writes past them 58.
 template <int GROUP>
 __global__ __launch_bounds__(256) void quantize_w4_kernel(const float* __restrict__ src, long ld, int rows, int cols,
                                                           unsigned per_row, unsigned char* __restrict__ codes,
@@ -161,7 +162,9 @@ __device__ __forceinline__ void store_y(const W4Args& a, long at, float y) {
 // A lane keeps the X of one unit (32 columns) of each row in registers as fp32 and walks down the rows of W: 16 bytes of
 // codes and a scale per row, converted two at a time and multiplied by fused multiply-adds.  Sixty-four lanes are 2048
 // columns: `kw` wavefronts lie side by side along K (a longer K takes several rounds), a shorter K has `lanes` lanes to
-// a row and several rows to a wavefront.  B loads of W are on their way while the B before are worked on.
+// a row and several rows to a wavefront.  B loads of W are on their way while the B before are worked on.  Bound by memory:
+// 1 x 16384 x 8192 in bf16 12.6 us = 5.5 TB/s, in fp32 14.4.  Matrix instructions, which round up to 16 rows, took 17.5; from
+// three rows on they are the faster ones (4 x 16384 x 8192 20.6 us here 31.6, 3 x 4096 x 4096 6.1 and 6.5).
 template <int CTRL>
 __device__ __forceinline__ float add_dpp(float x) {
     const int y = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true);
@@ -358,8 +361,8 @@ __global__ __launch_bounds__(64 * WAVES) void gemv_w4_kernel(const W4Args a, con
 // (16 x 16 x 32), so that a step's 32 columns lie in one group and the sum over a group takes one scale.  Columns of
 // workgroups start at different chunks of a slice: rows of W are often a power of two apart, and workgroups that walk
 // them in step would all ask the same few memory channels.
-//   Times (groups of 64): 16 x 16384 x 8192 24.9 us = 2.9 TB/s of W; left out by turns, X costs 7 us of it, matrix instructions
-// and conversions 4.5, and W, two launches and the join the rest.  24 x 4100 x 4090 14.5 us: X 4, the second
+//   Times (groups of 64): 16 x 16384 x 8192 24.1 us = 3.0 TB/s of W; left out by turns, X costs 7 us of it, matrix instructions
+// and conversions 4.5, and W, two launches and the join the rest.  24 x 4100 x 4090 14.3 us: X 4, the second
 // launch and the join 4.5, the rest a chain that is too short to overlap.  64 x 16384 x 8192 60 us, in bf16 35 = 490 TFLOP/s.
 // Scales that each wavefront loads for itself, chunk by chunk (16 lines for 64 bytes of each row), had cost 5 us of
 // 8 x 16384 x 8192 in bf16 (18.9 us); sixteen wavefronts to a workgroup, or a whole slice of W ahead, gained nothing.
@@ -506,8 +509,10 @@ constexpr int slice_chunks(int r, int mt, bool x_bf16) { return r == 4 ? 16 : mt
 constexpr int slice_scales(int slice, int group) { return slice * (128 / group); }
 constexpr int scales_pitch(int slice, int group) { return slice_scales(slice, group) * 2 + 16; }
 
+// X in fp32 leaves room in LDS for one workgroup on a CU, two wavefronts to a SIMD: said here, the compiler spends the registers
+// (16 x 16384 x 8192 24.1 us for 24.9, 24 x 4100 x 4090 14.3 for 14.6)
 template <int R, int MT, int NT, bool XBF, int GROUP>
-__global__ __launch_bounds__(64 * WAVES) void gemm_w4_kernel(const W4Args a, const GemmShape g) {
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, XBF || R == 4 ? 8 : 2))) void gemm_w4_kernel(const W4Args a, const GemmShape g) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     constexpr int PARTS = XBF ? 1 : 3, STEPS = GROUP / 32, SLICE = slice_chunks(R, MT, XBF), PIECES = R * MT * SLICE / 32;
     constexpr int SCALES = slice_scales(SLICE, GROUP), COUNT = SCALES < 8 ? SCALES : 8, RUNS = SCALES / COUNT, PITCH = scales_pitch(SLICE, GROUP);
