@@ -798,7 +798,8 @@ GemmPlan plan_gemm(int M, int N, int K, bool x_bf16) {
         for (int nt = 1; nt <= 2; nt++)
             for (int log_kw = 0; log_kw <= 3 && slice >> log_kw >= DEPTH && chunks >> log_kw; log_kw++) {
                 const int columns = 16 * nt * (WAVES >> log_kw);
-                const long blocks = ((long)N + columns - 1) / columns * m_blocks;
+                const long n_blocks = ((long)N + columns - 1) / columns, blocks = n_blocks * m_blocks;
+                if (n_blocks >= 1L << 23) continue;  // a launch has fewer than 2^32 threads in a row; 256 columns always do
                 // as many parts as there are CUs for, half or a quarter of them, and one
                 for (long want = std::min(std::min(64L, (long)chunks), std::max(1L, CUS / blocks)), turn = 0; turn < 4; turn++) {
                     const int parts = turn == 3 ? 1 : (int)(want >> turn);
