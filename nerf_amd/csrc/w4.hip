@@ -354,18 +354,18 @@ __global__ __launch_bounds__(64 * WAVES) void gemv_w4_kernel(const W4Args a, con
 // chunks of 128 columns.
 //   X: a slice of the rows' columns is put in LDS as matrix operands, once for all wavefronts: bf16 as it is, fp32 as
 // three bf16 numbers that add up to it exactly (its upper, middle and lower 8 significant bits, cut off), with one matrix
-// instruction each.  Codes are bf16 numbers exactly, so products are exact and sums are fp32.  The next slice is on its
-// way in registers while one is worked on.
+// instruction each.  Codes are bf16 numbers exactly, so products are exact and sums are fp32.  The slice after the next is
+// on its way in registers while one is worked on.
 //   W: per chunk a lane loads 16 bytes (one unit of 32 columns) of one of 16 rows straight to registers, DEPTH chunks
 // ahead; four lane swaps turn the four units that four lanes hold of a row into the four steps of a matrix instruction
 // (16 x 16 x 32), so that a step's 32 columns lie in one group and the sum over a group takes one scale.  Columns of
 // workgroups start at different chunks of a slice: rows of W are often a power of two apart, and workgroups that walk
 // them in step would all ask the same few memory channels.
-//   Times (groups of 64): 16 x 16384 x 8192 24.1 us = 3.0 TB/s of W; left out by turns, X costs 7 us of it, matrix instructions
-// and conversions 4.5, and W, two launches and the join the rest.  24 x 4100 x 4090 14.3 us: X 4, the second
-// launch and the join 4.5, the rest a chain that is too short to overlap.  64 x 16384 x 8192 60 us, in bf16 35 = 490 TFLOP/s.
+//   Times (groups of 64): 16 x 16384 x 8192 24.5 us = 2.9 TB/s of W; left out by turns, X costs 7 us of it, matrix instructions
+// and conversions 4.5, and W, two launches and the join the rest.  24 x 4100 x 4090 14.2 us: X 4, the second
+// launch and the join 4.5, the rest a chain that is too short to overlap.  64 x 16384 x 8192 59 us, in bf16 34 = 510 TFLOP/s.
 // Scales that each wavefront loads for itself, chunk by chunk (16 lines for 64 bytes of each row), had cost 5 us of
-// 8 x 16384 x 8192 in bf16 (18.9 us); sixteen wavefronts to a workgroup, or a whole slice of W ahead, gained nothing.
+// 8 x 16384 x 8192 in bf16 (17.9 us); sixteen wavefronts to a workgroup, or a whole slice of W ahead, gained nothing.
 // eight codes as eight bf16
 __device__ __forceinline__ bf16x8 values8_bf16(unsigned c) {
     const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, 1.0f, 1);
@@ -493,18 +493,21 @@ struct Scales {
 struct GemmShape {
     int log_kw;        // 2^log_kw wavefronts split the contraction: 1, 2, 4 or 8
     int split_chunks;  // chunks of one part of the contraction (gridDim.z parts), a multiple of a slice
-    int scales_at;     // bytes of LDS before the scales
+    int scales_at;     // bytes of a slice in LDS before its scales
+    int slice_bytes;   // bytes from one slice to the other where there are two, else 0
     float* partial;    // [parts][M][N], or null: one part, stored to Y
 };
 
 constexpr int CUS = 256;
 constexpr int DEPTH = 2;  // chunks of W on their way to a wavefront
 
-// Chunks of a slice, of X in R MT rows and of the scales: few enough that X in fp32 leaves room in LDS and that parts of the
-// contraction come out even (24 x 4100 x 4090: 14.4 us with 2, 15.6 with 4), and enough to cover the time of a read while
-// a slice is worked on (16 x 16384 x 8192: 24.5 us with 8, 25.6 with 4; 32 x 16384 x 8192 in bf16 with half of the parts:
-// 26 with 4, 33 with 2).
-constexpr int slice_chunks(int r, int mt, bool x_bf16) { return r == 4 ? 16 : mt == 1 ? 8 : x_bf16 ? 4 : 2; }
+// Chunks of a slice, of X in R MT rows and of the scales.  LDS holds two slices where it has room: the next one is put there
+// by some wavefronts while others still work on this one, and a slice costs one barrier instead of two (against one slice
+// of twice the length: 8 x 16384 x 8192 in bf16 17.9 us for 18.8, 32 x 16384 x 8192 37 for 39, 16 x 512 x 512 4.2 for 4.9, but
+// 6 x 200 x 16000 9.6 for 8.8).  Up to four rows in fp32 their eight wavefronts along the contraction need long slices.
+constexpr int slice_chunks(int r, int mt, bool x_bf16) { return r == 4 ? 16 : mt == 1 ? (x_bf16 ? 8 : 4) : x_bf16 ? 4 : 2; }
+// whether LDS has room for two slices
+constexpr bool two_slices(int r, int mt, bool x_bf16) { return r == 16 && (x_bf16 || mt <= 2); }
 // scales of a row in a slice; bytes from row to row in LDS
 constexpr int slice_scales(int slice, int group) { return slice * (128 / group); }
 constexpr int scales_pitch(int slice, int group) { return slice_scales(slice, group) * 2 + 16; }
@@ -561,7 +564,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, X
     // A thread's pieces of a slice: SLICE * 16 pieces in a row, R MT SLICE * 16 = PIECES * 512 of them.  A piece that holds the
     // row's last columns and others past them is put together by itself.
     Piece<XBF> piece[PIECES];
-    auto at_piece = [&](int r, int p) { return lds + (p / 4) * STEP_BYTES + (r / R) * TILE_BYTES + ((p % 4) * R + r % R) * 16; };
+    auto at_piece = [&](char* to, int r, int p) { return to + (p / 4) * STEP_BYTES + (r / R) * TILE_BYTES + ((p % 4) * R + r % R) * 16; };
     auto load_x = [&](int base) {
 #pragma unroll
         for (int k = 0; k < PIECES; k++) {
@@ -570,7 +573,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, X
             if (r < rows && col + 8 <= a.K) piece[k].load((const char*)a.X + (m0 + r) * a.ldx * (XBF ? 2 : 4), col);
         }
     };
-    auto stage_x = [&](int base) {
+    auto stage_x = [&](char* to, int base) {
         const int width = min(SLICE, end - base) * 16;  // pieces of a row that are looked at
 #pragma unroll
         for (int k = 0; k < PIECES; k++) {
@@ -578,7 +581,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, X
             if (r < rows && p < width && (col + 8 <= a.K || col >= a.K)) {
                 u32x4 o[PARTS];
                 piece[k].operands(o);
-                char* at = at_piece(r, p);
+                char* at = at_piece(to, r, p);
 #pragma unroll
                 for (int part = 0; part < PARTS; part++) *reinterpret_cast<u32x4*>(at + part * PART_BYTES) = o[part];
             }
@@ -594,14 +597,14 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, X
                     if constexpr (XBF) h[0] = (unsigned)((const unsigned short*)a.X)[from] << 16;
                     else split3_any(((const unsigned*)a.X)[from], h[0], h[1], h[2]);
                 }
-                char* at = at_piece(r, ragged / 8 - base * 16) + (q % 8) * 2;
+                char* at = at_piece(to, r, ragged / 8 - base * 16) + (q % 8) * 2;
 #pragma unroll
                 for (int part = 0; part < PARTS; part++) *reinterpret_cast<unsigned short*>(at + part * PART_BYTES) = h[part] >> 16;
             }
         }
     };
     // rows past the end are read as what LDS holds there, or as the last row where R < 16: their sums are not stored
-    const char* xlane = lds + (lj * R + min(ln, R - 1)) * 16;
+    const int xlane = (lj * R + min(ln, R - 1)) * 16;
 
     // the scales of the slice, of all rows of W of the workgroup: read in runs along a row, once for the wavefronts that
     // split the contraction, and one slice ahead like X
@@ -621,14 +624,14 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, X
             }
         }
     };
-    auto stage_scales = [&](int base) {
+    auto stage_scales = [&](char* to, int base) {
 #pragma unroll
         for (int k = 0; k < SCALE_TURNS; k++) {
             int row, run;
-            if (scales_of(k, row, run)) scales[k].put(lds + g.scales_at + row * PITCH + run * COUNT * 2, base * (128 / GROUP) + run * COUNT, a.groups);
+            if (scales_of(k, row, run)) scales[k].put(to + g.scales_at + row * PITCH + run * COUNT * 2, base * (128 / GROUP) + run * COUNT, a.groups);
         }
     };
-    const char* slane = lds + g.scales_at + (wn * 16 * NT + ln) * PITCH;
+    const int slane = g.scales_at + (wn * 16 * NT + ln) * PITCH;
 
     u32x4 w[DEPTH][NT];
     load_scales(first);
@@ -637,15 +640,15 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, X
 #pragma unroll
         for (int d = 0; d < DEPTH; d++) load(w[d], d);
     }
-    auto chunk = [&](const u32x4* w, int turn, int base) {
+    auto chunk = [&](const char* slice, const u32x4* w, int turn, int base) {
         const int at = chunk_of(turn) - base;
-        const char* xs = xlane + at * (4 * STEP_BYTES);
+        const char* xs = slice + xlane + at * (4 * STEP_BYTES);
         u32x4 codes[NT];
         float scales[NT][128 / GROUP];
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             codes[t] = transpose4(w[t]);
-            const char* from = slane + t * 16 * PITCH + at * (256 / GROUP);
+            const char* from = slice + slane + t * 16 * PITCH + at * (256 / GROUP);
             if constexpr (GROUP == 128) {
                 scales[t][0] = bf16_to_f32(*reinterpret_cast<const unsigned short*>(from));
             } else {
@@ -685,29 +688,52 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, X
         }
     };
     int turn = 0;
-    for (int base = first - SLICE; base < end; base += SLICE) {  // the first time round there is no slice yet
-        const bool more = base + SLICE < end;
-        if (more && base >= first) {
-            load_scales(base + SLICE);
-            load_x(base + SLICE);
-        }
-        if (base >= first) {
-            const int stop = min(turns_all, turn + (1 << log_turns));
-            // a whole slice has a multiple of DEPTH turns
-            for (; turn < stop; turn += DEPTH) {
+    auto work_on = [&](const char* slice, int base) {
+        const int stop = min(turns_all, turn + (1 << log_turns));
+        // a whole slice that others follow has a multiple of DEPTH turns
+        for (; turn < stop; turn += DEPTH) {
 #pragma unroll
-                for (int d = 0; d < DEPTH; d++) {
-                    if (turn + d < stop) chunk(w[d], turn + d, base);
-                    load(w[d], turn + d + DEPTH);
-                    asm volatile("" ::: "memory");  // the loads stay here, turns ahead of their use
-                }
+            for (int d = 0; d < DEPTH; d++) {
+                if (turn + d < stop) chunk(slice, w[d], turn + d, base);
+                load(w[d], turn + d + DEPTH);
+                asm volatile("" ::: "memory");  // the loads stay here, turns ahead of their use
             }
-            __syncthreads();
         }
-        if (more) {
-            stage_scales(base + SLICE);
-            stage_x(base + SLICE);
+    };
+    // the first time round there is no slice to work on yet
+    if constexpr (two_slices(R, MT, XBF)) {
+        int here = g.slice_bytes, other = 0;
+        for (int base = first - SLICE; base < end; base += SLICE) {
+            if (base + SLICE < end) {
+                stage_scales(lds + other, base + SLICE);
+                stage_x(lds + other, base + SLICE);
+            }
+            if (base + 2 * SLICE < end) {
+                load_scales(base + 2 * SLICE);
+                load_x(base + 2 * SLICE);
+            }
+            if (base >= first) work_on(lds + here, base);
             __syncthreads();
+            const int before = here;
+            here = other;
+            other = before;
+        }
+    } else {
+        for (int base = first - SLICE; base < end; base += SLICE) {
+            const bool more = base + SLICE < end;
+            if (more && base >= first) {
+                load_scales(base + SLICE);
+                load_x(base + SLICE);
+            }
+            if (base >= first) {
+                work_on(lds, base);
+                __syncthreads();
+            }
+            if (more) {
+                stage_scales(lds, base + SLICE);
+                stage_x(lds, base + SLICE);
+                __syncthreads();
+            }
         }
     }
 
@@ -770,8 +796,8 @@ __global__ __launch_bounds__(256) void join_w4_kernel(const W4Args a, const floa
 struct Costs {
     float x, weight, product, read, slice, join, part, value;
 };
-constexpr Costs F32_COSTS = {1.35e-4f, 2.4e-5f, 1.3e-5f, 0.0f, 0.36f, 4.0f, 0.09f, 3.1e-6f};
-constexpr Costs BF16_COSTS = {1.33e-5f, 7.9e-6f, 7.6e-6f, 4.4e-6f, 0.36f, 2.0f, 0.07f, 1.4e-6f};
+constexpr Costs F32_COSTS = {7.5e-5f, 7.7e-6f, 1.14e-5f, 0.0f, 0.44f, 2.3f, 0.075f, 2.7e-6f};
+constexpr Costs BF16_COSTS = {2.1e-5f, 5.5e-6f, 7.6e-6f, 4.4e-6f, 0.36f, 2.36f, 0.07f, 1.4e-6f};
 
 struct GemmPlan {
     int r, mt, nt, log_kw, parts, split_chunks;
@@ -780,13 +806,14 @@ struct GemmPlan {
 // The shape of a launch is the one whose estimated time is least (us on 256 CUs, a workgroup at a time on each): so much for
 // a value of X (brought in, split, put in LDS), for a weight (brought in and converted), for a weight and a tile of rows
 // (multiplied), for a tile of X read from LDS for 16 NT columns, for a slice, for the second kernel that joins parts, for a part,
-// and for a value of one (written and read).  The numbers are fitted to 2100 measured launches of 37 shapes (3 to 200
+// and for a value of one (written and read).  The numbers are fitted to 3600 measured launches of 41 shapes (3 to 200
 // rows, 200 to 32768 columns, K from 500 to 16384) so that the shapes they find are the fastest ones measured: they
-// are within 11 % of those, and 24 x 4100 x 4090 in bf16 within 16 (12.9 us for 11.2).  What decides, with both sides measured:
-//   rows to a workgroup: 64 x 16384 x 8192 61 us with 64 and 70 with 16, but 64 x 512 x 512 12.3 and 5.1
-//   columns of a wavefront, 16 or 32: 16 x 16384 x 8192 30.4 and 25.4 us, but 4 x 512 x 512 4.3 and 5.1
-//   wavefronts along the contraction: 3 x 4096 x 4096 6.2, 7.6 and 29 us with 8, 4 and 1; 16 x 16384 x 8192 25.4 with 1, 28.5 with 2
-//   parts: 24 x 4100 x 4090 14.4 us with 6 (a join among them), 15.7 with 4; 64 x 4096 x 4096 in bf16 10.8 with 1, 12.5 with 3
+// are within 5 % of those for 36 of them and within 10 % for all.  What decides, with both sides measured (X in fp32):
+//   rows to a workgroup: 64 x 16384 x 8192 61 us with 64 and 72 with 16, but 64 x 512 x 512 4.3 with 16 and 7.6 with 32
+//   columns of a wavefront, 16 or 32: 16 x 16384 x 8192 31.1 and 25.8 us, but 64 x 512 x 512 4.3 and 4.9
+//   wavefronts along the contraction: 3 x 4096 x 4096 6.2, 7.5, 10.5 and 16.6 us with 8, 4, 2 and 1; 16 x 16384 x 8192 25.8 with 1
+// and 30.6 with 2
+//   parts: 24 x 4100 x 4090 38.6, 24.3, 14.4 and 18.6 us with 1, 2, 6 and 12
 GemmPlan plan_gemm(int M, int N, int K, bool x_bf16) {
     GemmPlan best = {};
     const int chunks = K / 128 + (K % 128 != 0), r = M <= 4 ? 4 : 16;
@@ -796,7 +823,7 @@ GemmPlan plan_gemm(int M, int N, int K, bool x_bf16) {
         const int slice = slice_chunks(r, mt, x_bf16);
         const long m_blocks = (M + r * mt - 1L) / (r * mt);
         for (int nt = 1; nt <= 2; nt++)
-            for (int log_kw = 0; log_kw <= 3 && slice >> log_kw >= DEPTH && chunks >> log_kw; log_kw++) {
+            for (int log_kw = 0; log_kw <= 3 && slice >> log_kw && chunks >> log_kw; log_kw++) {
                 const int columns = 16 * nt * (WAVES >> log_kw);
                 const long n_blocks = ((long)N + columns - 1) / columns, blocks = n_blocks * m_blocks;
                 if (n_blocks >= 1L << 23) continue;  // a launch has fewer than 2^32 threads in a row; 256 columns always do
@@ -806,6 +833,7 @@ GemmPlan plan_gemm(int M, int N, int K, bool x_bf16) {
                     if (parts < 1 || (parts == 1 && turn < 3)) continue;
                     int split = (chunks + parts - 1) / parts;
                     if (parts > 1 && split > slice) split = (split + slice - 1) / slice * slice;
+                    if (split > slice && slice >> log_kw < DEPTH) continue;
                     const int used = (chunks + split - 1) / split;
                     const float depth = (float)std::min(split * 128L, (long)K), slices = (float)((split + slice - 1) / slice);
                     const float work = depth * (of.x * std::min(M, r * mt) + columns * (of.weight + mt * (of.product + of.read / nt))) + of.slice * slices;
@@ -826,8 +854,10 @@ hipError_t launch_gemm(const W4Args& a, const GemmPlan& p, float* partial) {
     constexpr int PARTS = XBF ? 1 : 3, SLICE = slice_chunks(R, MT, XBF);
     const size_t x_bytes = (size_t)std::min(SLICE, p.split_chunks) * 4 * (PARTS * MT * R * 64 + 16);
     const long columns = 16L * NT * (WAVES >> p.log_kw);
-    const size_t bytes = std::max(x_bytes + (size_t)columns * scales_pitch(SLICE, GROUP), (size_t)WAVES * NT * 64 * 16);
-    const GemmShape shape = {p.log_kw, p.split_chunks, (int)x_bytes, p.parts > 1 ? partial : nullptr};
+    const size_t slice_bytes = x_bytes + (size_t)columns * scales_pitch(SLICE, GROUP);
+    const bool two = two_slices(R, MT, XBF) && p.split_chunks > SLICE;
+    const size_t bytes = std::max(slice_bytes * (two ? 2 : 1), (size_t)WAVES * NT * 64 * 16);
+    const GemmShape shape = {p.log_kw, p.split_chunks, (int)x_bytes, two ? (int)slice_bytes : 0, p.parts > 1 ? partial : nullptr};
     constexpr long MOST = 65535L * R * MT;  // rows of a launch: gridDim.y has 16 bits
     for (long m = 0; m < a.M; m += MOST) {
         W4Args some = a;
