@@ -50,8 +50,9 @@ __device__ __forceinline__ long piece_of(unsigned id, unsigned per_row, int rows
 }
 
 // A thread takes eight consecutive columns of a row; the 4, 8 or 16 threads of a group are neighbours in a row of sixteen
-// lanes (a row of W has whole groups of threads).  Bound by memory: 8192 x 8192 57 us = 5.3 TB/s; two such pieces to a thread
-// 58, reads past the caches 60, writes past them 58.
+// lanes (a row of W has whole groups of threads).  Bound by memory: 8192 x 8192 53.6 us = 5.7 TB/s; two such pieces to a
+// thread 56, four columns to a thread, so that a load takes whole lines in a row, 63 (57.5 with two pieces), reads past the
+// caches 55.  Vector work is next (seven comparisons to a weight instead of a quotient: 57.5).
 template <int GROUP>
 __global__ __launch_bounds__(256) void quantize_w4_kernel(const float* __restrict__ src, long ld, int rows, int cols,
                                                           unsigned per_row, unsigned char* __restrict__ codes,
@@ -85,24 +86,26 @@ __global__ __launch_bounds__(256) void quantize_w4_kernel(const float* __restric
     s += 6.0f * bf16_to_f32((unsigned short)s) < largest;
     const bool bad = top >= 0x7F800000u;
     if (row >= rows) return;
-    // The borders between codes are multiples of the scale and exact in fp32; a tie takes the even code.  Which side of three
-    // borders a weight is on gives the three bits.  Without a scale (a group of zeros, or one that is not finite) every
-    // border is out of reach.
-    const float scale = bad || top == 0 ? INFINITY : bf16_to_f32((unsigned short)s);
-    const float b1 = 0.25f * scale, b2 = 0.75f * scale, b3 = 1.25f * scale, b4 = 1.75f * scale, b5 = 2.5f * scale, b6 = 3.5f * scale,
-                b7 = 5.0f * scale;
-    unsigned word = 0;
+    // The quotient by the scale, as its fp32 rounding, and the conversion to nearest with ties to even decide as the weights
+    // themselves do: a weight that is not on a border between codes (a multiple of the scale with 12 bits at most) is a step
+    // of its own away from it, 2^-24 and more, and the scale's 8 bits leave the quotient 2^-32 farther from the border than
+    // half a step of fp32.  One correction of a product with the reciprocal is as near as 2^-45.  Powers of two are taken out
+    // first, for scales whose reciprocal would leave fp32's range.
+    const float scale = bf16_to_f32((unsigned short)s), part = __builtin_amdgcn_frexp_mantf(scale);
+    const int exponent = __builtin_amdgcn_frexp_expf(scale);
+    const float inverse = top == 0 ? 0.0f : __builtin_amdgcn_rcpf(part);
+    float q[8];
 #pragma unroll
     for (int k = 0; k < 8; k++) {
-        const float a = bad ? 0.0f : fabsf(x[k]);
-        const bool four = a >= b4, two = a >= (four ? b6 : b2);
-        const float lower = four ? b5 : b1, upper = four ? b7 : b3;
-        const bool one = a > (two ? upper : lower);
-        unsigned c = four ? 4u : 0u;
-        c = c + (two ? 2u : 0u) + (one ? 1u : 0u);
-        if (c && x[k] < 0.0f) c |= 8;
-        word |= c << (4 * k);
+        const float w = __builtin_amdgcn_ldexpf(x[k], -exponent), near = w * inverse;
+        q[k] = __builtin_fmaf(__builtin_fmaf(-near, part, w), inverse, near);
     }
+    unsigned word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, q[0], q[1], 1.0f, 0);
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, q[2], q[3], 1.0f, 1);
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, q[4], q[5], 1.0f, 2);
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, q[6], q[7], 1.0f, 3);
+    const unsigned some = (word | word >> 1 | word >> 2) & 0x11111111u;  // codes that are not zero: only they keep a sign
+    word = bad ? 0u : word & (0x77777777u | some << 3);
     if ((long)place * 4 < row_bytes) *reinterpret_cast<unsigned*>(codes + row * row_bytes + (long)place * 4) = word;
     if (place % (GROUP / 8) == 0) scales[row * groups + place / (GROUP / 8)] = bad ? 0x7FC0 : (unsigned short)s;
 }

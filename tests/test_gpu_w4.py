@@ -77,6 +77,34 @@ def test_quantize_extremes(gpu):
     assert np.isnan(ref.from_bf16(scales.read())[~fine]).all() and np.isfinite(ref.from_bf16(scales.read())[fine]).all()
 
 
+@pytest.mark.parametrize("power", [-133, -126, -40, 0, 60, 125])
+def test_quantize_next_to_borders(gpu, power):
+    """every scale mantissa of 8 bits, and weights on each border between codes and up to three fp32 numbers beside it"""
+    from nerf_amd._lib import lib
+    bits = np.arange(128, 256, dtype=np.float64) * 2.0 ** (power - 7)
+    scale = ref.from_bf16((bits.astype(np.float32).view(np.uint32) >> 16).astype(np.uint16)).astype(np.float32)  # cut where subnormal
+    borders = np.float32([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])
+    rows = []
+    for s in scale:
+        if 6.0 * float(s) > 3.4e38:
+            continue
+        at = (borders * s).astype(np.float32)  # exact, but for subnormal scales: numbers like others there
+        w = [s * np.float32(6)] + [v for b in at for v in (b, -b)]
+        for b in at:
+            up = down = b
+            for _ in range(3):
+                up, down = np.nextafter(up, np.float32(np.inf)), np.nextafter(down, np.float32(0))
+                w += [up, -down, -up, down]
+        rows.append(np.float32(w + [0.0] * (-len(w) % 128)))
+    w = np.stack(rows)
+    n, k = w.shape
+    assert k == 128
+    d, codes, scales = Guarded(w), Guarded(np.zeros((n, 64), np.uint8)), Guarded(np.zeros((n, 1), np.uint16))
+    assert lib.nerf_quantize_w4(d.ptr, k, n, k, 128, codes.ptr, scales.ptr) == 0
+    want_codes, want_scales = ref.quantize_w4(w, 128)
+    assert np.array_equal(scales.read(), want_scales) and np.array_equal(codes.read(), want_codes)
+
+
 def run(x, codes, scales, group, n, k, x_bf16, y_bf16, epilogue, ldx=None, ldy=None, shift=0):
     from nerf_amd._lib import lib
     from nerf_amd.api import DeviceArray
