@@ -151,7 +151,9 @@ SHAPES = [(1, 1, 1), (1, 3, 31), (1, 17, 33), (2, 64, 32), (1, 512, 512), (1, 10
           (100, 130, 300), (129, 17, 64), (1, 4099, 96), (2, 5000, 40), (64, 1030, 64),
           # long rows in several rounds or slices, and rows of W that end inside a wavefront's share
           (2, 70, 16384), (1, 5, 40000), (2, 9, 33000), (1, 2000, 1000), (2, 700, 8), (1, 70000, 24), (3, 35, 20000), (20, 40, 5000),
-          (64, 9000, 200)]
+          (64, 9000, 200),
+          # many columns and several slices: the most LDS
+          (64, 8300, 1100), (33, 17000, 700), (4, 9000, 5000), (16, 16500, 1300)]
 
 
 @pytest.mark.parametrize("group", [32, 64, 128])
