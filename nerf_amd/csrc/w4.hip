@@ -524,8 +524,11 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, X
     constexpr int SCALES = slice_scales(SLICE, GROUP), COUNT = SCALES < 8 ? SCALES : 8, RUNS = SCALES / COUNT, PITCH = scales_pitch(SLICE, GROUP);
     constexpr int SCALE_TURNS = (16 * NT * WAVES * RUNS + 64 * WAVES - 1) / (64 * WAVES);
     // LDS: [step of 32 columns][part][tile of R rows][unit of 8 columns][row], 16 bytes each: a wavefront reads an operand as
-    // one run; the steps are 16 bytes further apart, so that a run of a row's pieces is written to different banks
-    constexpr int TILE_BYTES = R * 64, PART_BYTES = MT * TILE_BYTES, STEP_BYTES = PARTS * PART_BYTES + 16;
+    // one run; the steps are 16 bytes further apart, and the upper two units' rows in another order (row ^ 4), so that a run of
+    // a row's pieces is written to different banks (half of the conflicts: 64 x 16384 x 8192 59 -> 55.5 us).  An order that differs
+    // in each unit makes reads collide, and threads that take pieces below each other read rows that are often a power of
+    // two apart: both slower
+    constexpr int TILE_BYTES = R * 64, PART_BYTES = MT * TILE_BYTES, STEP_BYTES = PARTS * PART_BYTES + 16, SWIZZLE = R == 16 ? 4 : 0;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ln = lane & 15, lj = lane >> 4;
     const int kw = 1 << g.log_kw, columns = WAVES >> g.log_kw;  // wavefronts along the contraction, along N
@@ -567,7 +570,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, X
     // A thread's pieces of a slice: SLICE * 16 pieces in a row, R MT SLICE * 16 = PIECES * 512 of them.  A piece that holds the
     // row's last columns and others past them is put together by itself.
     Piece<XBF> piece[PIECES];
-    auto at_piece = [&](char* to, int r, int p) { return to + (p / 4) * STEP_BYTES + (r / R) * TILE_BYTES + ((p % 4) * R + r % R) * 16; };
+    auto at_piece = [&](char* to, int r, int p) { return to + (p / 4) * STEP_BYTES + (r / R) * TILE_BYTES + ((p % 4) * R + (r % R ^ (p % 4 / 2 * SWIZZLE))) * 16; };
     auto load_x = [&](int base) {
 #pragma unroll
         for (int k = 0; k < PIECES; k++) {
@@ -607,7 +610,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, X
         }
     };
     // rows past the end are read as what LDS holds there, or as the last row where R < 16: their sums are not stored
-    const int xlane = (lj * R + min(ln, R - 1)) * 16;
+    const int xlane = (lj * R + (min(ln, R - 1) ^ (lj / 2 * SWIZZLE))) * 16;
 
     // the scales of the slice, of all rows of W of the workgroup: read in runs along a row, once for the wavefronts that
     // split the contraction, and one slice ahead like X
