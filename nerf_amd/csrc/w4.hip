@@ -364,11 +364,11 @@ __global__ __launch_bounds__(64 * WAVES) void gemv_w4_kernel(const W4Args a, con
 // (16 x 16 x 32), so that a step's 32 columns lie in one group and the sum over a group takes one scale.  Columns of
 // workgroups start at different chunks of a slice: rows of W are often a power of two apart, and workgroups that walk
 // them in step would all ask the same few memory channels.
-//   Times (groups of 64): 16 x 16384 x 8192 24.5 us = 2.9 TB/s of W; left out by turns, X costs 7 us of it, matrix instructions
-// and conversions 4.5, and W, two launches and the join the rest.  24 x 4100 x 4090 14.2 us: X 4, the second
-// launch and the join 4.5, the rest a chain that is too short to overlap.  64 x 16384 x 8192 59 us, in bf16 34 = 510 TFLOP/s.
+//   Times (groups of 64): 16 x 16384 x 8192 23.6 us = 3.0 TB/s of W; left out by turns, X costs 7 us of it, matrix instructions
+// and conversions 4.5, and W, two launches and the join the rest.  24 x 4100 x 4090 13.8 us: X 4, the second
+// launch and the join 4.5, the rest a chain that is too short to overlap.  64 x 16384 x 8192 55.5 us, in bf16 33 = 520 TFLOP/s.
 // Scales that each wavefront loads for itself, chunk by chunk (16 lines for 64 bytes of each row), had cost 5 us of
-// 8 x 16384 x 8192 in bf16 (17.9 us); sixteen wavefronts to a workgroup, or a whole slice of W ahead, gained nothing.
+// 8 x 16384 x 8192 in bf16 (17.6 us); sixteen wavefronts to a workgroup, or a whole slice of W ahead, gained nothing.
 // eight codes as eight bf16
 __device__ __forceinline__ bf16x8 values8_bf16(unsigned c) {
     const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, 1.0f, 1);
@@ -502,7 +502,9 @@ struct GemmShape {
 };
 
 constexpr int CUS = 256;
-constexpr int DEPTH = 2;  // chunks of W on their way to a wavefront
+// Chunks of W on their way to a wavefront: 4 x 16384 x 8192 23.9, 20.5 and 21.0 us with 1, 2 and 4, 8 x 16384 x 8192 in bf16
+// 18.2, 17.6 and 20.1, 16 x 512 x 512 4.06, 4.14 and 4.58: the loop is as many chunks long, and small products also wait for code.
+constexpr int DEPTH = 2;
 
 // Chunks of a slice, of X in R MT rows and of the scales.  LDS holds two slices where it has room: the next one is put there
 // by some wavefronts while others still work on this one, and a slice costs one barrier instead of two (against one slice
