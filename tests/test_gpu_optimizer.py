@@ -395,6 +395,33 @@ def test_no_plan_is_made_while_a_stream_is_captured(gpu):
         assert norm.item() == want.item() != 0.0
 
 
+def test_more_than_2_to_the_32_elements(gpu):
+    """one tensor longer than 32 bits count: equal elements stay equal to the end, and the norm counts them all"""
+    torch = pytest.importorskip("torch")
+    from nerf_amd._lib import lib
+    from nerf_amd.api import AdamW
+    n = 2 ** 32 + 1030
+    blocks = lib.nerf_adamw_state_blocks(n)
+    new = lambda count, t: torch.zeros(count, dtype=t, device="cuda")
+    w, g = new(n, torch.float32), torch.full((n,), 0.5, dtype=torch.bfloat16, device="cuda")
+    m, v, me, ve = new(n, torch.uint8), new(n, torch.uint8), new(blocks, torch.uint8), new(blocks, torch.uint8)
+    norm = new(1, torch.float32)
+    torch.cuda.synchronize()
+    plan = AdamW([dict(w=w.data_ptr(), g=g.data_ptr(), m=m.data_ptr(), v=v.data_ptr(), m_exp=me.data_ptr(), v_exp=ve.data_ptr(), n=n,
+                       g_bf16=True)], state_bits=8)
+    plan.grad_norm(norm.data_ptr())
+    plan.step(1, 1e-2)
+    torch.cuda.synchronize()
+    assert norm.item() == np.float32(0.5 * np.sqrt(n))
+    # m / (sqrt(v) + eps) times the corrections for the first step is 1 to a few roundings
+    assert abs(w[0].item() + 1e-2) <= 1e-2 * 16 * EPS32 + 1e-2 * 1e-8 / 0.5
+    for t in (w, m, v, me, ve):
+        assert bool((t == t[0]).all()) and t[0].item() != 0
+    plan.destroy()
+    del w, g, m, v, t
+    torch.cuda.empty_cache()
+
+
 def test_training_step_with_8_bit_states(gpu):
     """forward and backward of the trainer, the norm, and the clipped 8-bit step on the trainer's own arenas: three
     steps, each against the formula on the gradients and states the device held before it"""

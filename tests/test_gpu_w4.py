@@ -256,6 +256,31 @@ def test_more_rows_than_a_launch_takes(gpu):
     check(run(x, codes, scales, 32, n, k, False, False, 0), x.astype(np.float64), ref.dequantize_w4(codes, scales, k, 32), False, 0)
 
 
+def test_codes_past_four_gib(gpu):
+    """rows of W behind 2^32 bytes of codes, and their scales, in each kernel"""
+    torch = pytest.importorskip("torch")
+    from nerf_amd._lib import lib
+    n, k, group = 66000, 131072, 128
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    codes = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, device="cuda", generator=gen)
+    scales = torch.randint(0x3C00, 0x4000, (n, k // group), dtype=torch.int16, device="cuda", generator=gen)
+    assert codes.numel() > 2 ** 32
+    rows = [0, 1000, 65535, 65536, 65999]
+    w = ref.dequantize_w4(codes[rows].cpu().numpy(), scales[rows].cpu().numpy().view(np.uint16), k, group)
+    for m in (1, 3, 20):
+        x = torch.randn(m, k, device="cuda", generator=gen)
+        y = torch.empty(m, n, device="cuda")
+        size = lib.nerf_gemm_w4_workspace(m, n, k)
+        ws = torch.empty(size + 16, dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        assert lib.nerf_gemm_w4(x.data_ptr(), 0, k, codes.data_ptr(), scales.data_ptr(), group, y.data_ptr(), 0, n, m, n, k, 0,
+                                ws.data_ptr(), size) == 0
+        torch.cuda.synchronize()
+        check(y[:, rows].cpu().numpy(), x.cpu().numpy().astype(np.float64), w, False, 0)
+    del codes, scales, x, y, ws
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.parametrize("m", [1, 24])
 def test_graphs_and_streams(gpu, m):
     """quantize, a product (of 24 rows: with parts and their join) and dequantize in one graph on another stream than the
