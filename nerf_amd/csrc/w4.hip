@@ -30,10 +30,10 @@ __device__ __forceinline__ unsigned max_dpp(unsigned x) {
     return max(x, y);
 }
 
-// the eight values of a dword of codes
-__device__ __forceinline__ void values8(unsigned c, float* v) {
-    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 1);
-    const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 3);
+// the eight values of a dword of codes, times two: whole numbers, whose products with fp32 numbers are multiples of 2^-149
+__device__ __forceinline__ void doubles8(unsigned c, float* v) {
+    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 2.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 2.0f, 1);
+    const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 2.0f, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 2.0f, 3);
     v[0] = a[0]; v[1] = a[1]; v[2] = b[0]; v[3] = b[1];
     v[4] = d[0]; v[5] = d[1]; v[6] = e[0]; v[7] = e[1];
 }
@@ -282,7 +282,7 @@ __global__ __launch_bounds__(64 * WAVES) void gemv_w4_kernel(const W4Args a, con
 #pragma unroll
             for (int b = 0; b < B; b++) {
                 c[b] = next[b];
-                scale[b] = live ? bf16_to_f32(next_scale[b]) : 0.0f;
+                scale[b] = live ? bf16_to_f32(next_scale[b]) * 0.5f : 0.0f;
             }
             if (first + B < g.loads) load(first + B);
             asm volatile("" ::: "memory");  // the loads stay here, B rows ahead of their use
@@ -294,7 +294,7 @@ __global__ __launch_bounds__(64 * WAVES) void gemv_w4_kernel(const W4Args a, con
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
                     float v[8];
-                    values8(c[b][q], v);
+                    doubles8(c[b][q], v);
 #pragma unroll
                     for (int m = 0; m < M; m++)
 #pragma unroll
@@ -357,7 +357,8 @@ __global__ __launch_bounds__(64 * WAVES) void gemv_w4_kernel(const W4Args a, con
 // chunks of 128 columns.
 //   X: a slice of the rows' columns is put in LDS as matrix operands, once for all wavefronts: bf16 as it is, fp32 as
 // three bf16 numbers that add up to it exactly (its upper, middle and lower 8 significant bits, cut off), with one matrix
-// instruction each.  Codes are bf16 numbers exactly, so products are exact and sums are fp32.  The slice after the next is
+// instruction each.  What these leave over of a number below 2^-110 is seen as it is put there, and multiplied after the rest
+// (add_left_over).  Codes are bf16 numbers exactly, so products are exact and sums are fp32.  The slice after the next is
 // on its way in registers while one is worked on.
 //   W: per chunk a lane loads 16 bytes (one unit of 32 columns) of one of 16 rows straight to registers, DEPTH chunks
 // ahead; four lane swaps turn the four units that four lanes hold of a row into the four steps of a matrix instruction
@@ -395,6 +396,15 @@ __device__ __forceinline__ void split3_any(unsigned x, unsigned& hi, unsigned& m
     mid = lo = 0;
 }
 
+// A bf16 number has no bit below 2^-133, so the parts of a number below 2^-110 may leave something over, then the lower half of
+// `lo`: this much, times 2^32
+__device__ __forceinline__ float left_over(unsigned x) {
+    if ((x & 0x7FFFFFFFu) >= 0x08800000u) return 0.0f;  // 2^-110 and above, and what is not finite
+    unsigned hi, mid, lo;
+    split3(x, hi, mid, lo);
+    return (__builtin_bit_cast(float, lo) - __builtin_bit_cast(float, lo & 0xFFFF0000u)) * 0x1p32f;
+}
+
 // Eight consecutive values of a row of X as they lie in memory, and as one or three operands of eight bf16
 template <bool XBF>
 struct Piece {
@@ -412,28 +422,38 @@ struct Piece {
 #pragma unroll
         for (int k = 0; k < (XBF ? 1 : 2); k++) v[k] = u32x4{0, 0, 0, 0};
     }
-    __device__ __forceinline__ void operands(u32x4* o) const {
+    // the answer's lower half is not zero if the parts leave something over
+    __device__ __forceinline__ unsigned operands(u32x4* o) const {
         if constexpr (XBF) {
             o[0] = v[0];
+            return 0;
         } else {
-            unsigned hi[8], mid[8], lo[8];
-            float none = 0.0f;  // of finite numbers, times zero
+            unsigned hi[8], mid[8], lo[8], left = 0;
+            auto pack = [&] {
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const unsigned x = v[k / 4][k % 4];
-                split3(x, hi[k], mid[k], lo[k]);
-                none = __builtin_fmaf(__builtin_bit_cast(float, x), 0.0f, none);
+                for (int k = 0; k < 4; k++) {
+                    o[0][k] = upper_halves(hi[2 * k], hi[2 * k + 1]);
+                    o[1][k] = upper_halves(mid[2 * k], mid[2 * k + 1]);
+                    o[2][k] = upper_halves(lo[2 * k], lo[2 * k + 1]);
+                }
+            };
+#pragma unroll
+            for (int k = 0; k < 8; k++) split3(v[k / 4][k % 4], hi[k], mid[k], lo[k]);
+            pack();
+            float none = 0.0f;  // lo times zero: a NaN if any number is not finite
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const unsigned two = o[2][k];  // (a bit cast of the element itself reads the first one)
+                none = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, two), bf16x2{0, 0}, none, false);
             }
             if (none != 0.0f) {
 #pragma unroll
                 for (int k = 0; k < 8; k++) split3_any(v[k / 4][k % 4], hi[k], mid[k], lo[k]);
+                pack();
             }
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                o[0][k] = upper_halves(hi[2 * k], hi[2 * k + 1]);
-                o[1][k] = upper_halves(mid[2 * k], mid[2 * k + 1]);
-                o[2][k] = upper_halves(lo[2 * k], lo[2 * k + 1]);
-            }
+            for (int k = 0; k < 8; k++) left |= lo[k];
+            return left;
         }
     }
 };
@@ -517,11 +537,77 @@ constexpr bool two_slices(int r, int mt, bool x_bf16) { return r == 16 && (x_bf1
 constexpr int slice_scales(int slice, int group) { return slice * (128 / group); }
 constexpr int scales_pitch(int slice, int group) { return slice_scales(slice, group) * 2 + 16; }
 
+struct GemmArguments {  // as they lie in memory
+    W4Args a;
+    GemmShape g;
+};
+
+// The products with what the parts of X leave over, its 16 bits as two parts, slice by slice and nothing ahead: rare.  It
+// reads the arguments again, so that its needs take no registers from what runs before it: inside the main loop, as its second
+// time round, it cost every call 1 us.  Seeing that there is something costs 0.1 to 0.2 us (16 x 512 x 512 4.15 us without and
+// 4.28 with, 24 x 4100 x 4090 13.8 and 14.1, 64 x 16384 x 8192 57.8 and 59.3).
+template <int R, int MT, int NT, int GROUP>
+__device__ __forceinline__ void add_left_over(char* lds, f32x4 (&acc)[MT][NT]) {
+    constexpr int SLICE = slice_chunks(R, MT, false), TILE_BYTES = R * 64, PART_BYTES = MT * TILE_BYTES, STEP_BYTES = 2 * PART_BYTES + 16;
+    auto memory = (__attribute__((address_space(4))) const GemmArguments*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(memory));
+    const auto& a = memory->a;
+    const unsigned thread = threadIdx.x;
+    const int lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6), ln = lane & 15, lj = lane >> 4;
+    const int log_kw = memory->g.log_kw, kw = 1 << log_kw, wk = wave & (kw - 1);
+    const long n0 = ((long)blockIdx.x * (WAVES >> log_kw) + (wave >> log_kw)) * (16 * NT), m0 = (long)blockIdx.y * (R * MT);
+    const int rows = (int)min((long)(R * MT), a.M - m0), chunks = (a.K + 127) / 128, units = (a.K + 31) / 32;
+    const int first = blockIdx.z * memory->g.split_chunks, end = min(chunks, first + memory->g.split_chunks);
+#pragma unroll 1
+    for (int base = first; base < end; base += SLICE) {
+        const int width = min(SLICE, end - base) * 128;
+        __syncthreads();
+#pragma unroll 1
+        for (int q = thread; q < rows * width; q += 64 * WAVES) {
+            const int r = q / width, p = q % width, col = base * 128 + p;
+            const float x = col < a.K ? left_over(((const unsigned*)a.X)[(m0 + r) * a.ldx + col]) : 0.0f;
+            unsigned h[3];
+            split3(__builtin_bit_cast(unsigned, x), h[0], h[1], h[2]);
+            char* at = lds + (p / 32) * STEP_BYTES + (r / R) * TILE_BYTES + (p % 32 / 8 * R + r % R) * 16 + p % 8 * 2;
+            reinterpret_cast<unsigned short*>(at)[0] = h[0] >> 16;
+            reinterpret_cast<unsigned short*>(at + PART_BYTES)[0] = h[1] >> 16;
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (int c = base + wk; c < min(end, base + SLICE); c += kw) {
+            const char* xs = lds + (c - base) * (4 * STEP_BYTES) + (lj * R + min(ln, R - 1)) * 16;
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const long n = min(n0 + t * 16 + ln, (long)a.N - 1);
+                const u32x4 codes = transpose4(*reinterpret_cast<const u32x4*>(a.codes + n * a.row_bytes + (long)min(c * 4 + lj, units - 1) * 16));
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    float scale = c * 4 + s < units ? bf16_to_f32(a.scales[n * a.groups + (c * 4 + s) / (GROUP / 32)]) : 0.0f;
+                    if (!(fabsf(scale) < INFINITY)) scale = 0.0f;  // the sum has what it makes of it
+                    scale *= 0x1p-32f;  // loses bits where these products are below 2^-200
+                    const bf16x8 v = values8_bf16(codes[s]);
+#pragma unroll
+                    for (int i = 0; i < MT; i++) {
+                        const char* at = xs + s * STEP_BYTES + i * TILE_BYTES;
+                        f32x4 part = {0.f, 0.f, 0.f, 0.f};
+                        part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8*>(at + PART_BYTES), v, part, 0, 0, 0);
+                        part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8*>(at), v, part, 0, 0, 0);
+                        asm volatile("" ::: "memory");  // one at a time: few registers
+#pragma unroll
+                        for (int r = 0; r < 4; r++) acc[i][t][r] = __builtin_fmaf(part[r], scale, acc[i][t][r]);
+                    }
+                }
+            }
+        }
+    }
+}
+
 // X in fp32 leaves room in LDS for one workgroup on a CU, two wavefronts to a SIMD: said here, the compiler spends the registers
 // (16 x 16384 x 8192 24.1 us for 24.9, 24 x 4100 x 4090 14.3 for 14.6)
 template <int R, int MT, int NT, bool XBF, int GROUP>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, XBF || R == 4 ? 8 : 2))) void gemm_w4_kernel(const W4Args a, const GemmShape g) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ unsigned leaves[XBF ? 1 : WAVES];  // whether a wavefront's X leaves something over
     constexpr int PARTS = XBF ? 1 : 3, STEPS = GROUP / 32, SLICE = slice_chunks(R, MT, XBF), PIECES = R * MT * SLICE / 32;
     constexpr int SCALES = slice_scales(SLICE, GROUP), COUNT = SCALES < 8 ? SCALES : 8, RUNS = SCALES / COUNT, PITCH = scales_pitch(SLICE, GROUP);
     constexpr int SCALE_TURNS = (16 * NT * WAVES * RUNS + 64 * WAVES - 1) / (64 * WAVES);
@@ -582,13 +668,14 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, X
         }
     };
     auto stage_x = [&](char* to, int base) {
+        unsigned left = 0;
         const int width = min(SLICE, end - base) * 16;  // pieces of a row that are looked at
 #pragma unroll
         for (int k = 0; k < PIECES; k++) {
             const int q = threadIdx.x + k * 64 * WAVES, r = q / (SLICE * 16), p = q % (SLICE * 16), col = base * 128 + p * 8;
             if (r < rows && p < width && (col + 8 <= a.K || col >= a.K)) {
                 u32x4 o[PARTS];
-                piece[k].operands(o);
+                left |= piece[k].operands(o);
                 char* at = at_piece(to, r, p);
 #pragma unroll
                 for (int part = 0; part < PARTS; part++) *reinterpret_cast<u32x4*>(at + part * PART_BYTES) = o[part];
@@ -604,11 +691,15 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, X
                     const long from = (m0 + r) * a.ldx + col;
                     if constexpr (XBF) h[0] = (unsigned)((const unsigned short*)a.X)[from] << 16;
                     else split3_any(((const unsigned*)a.X)[from], h[0], h[1], h[2]);
+                    left |= XBF ? 0 : h[2];
                 }
                 char* at = at_piece(to, r, ragged / 8 - base * 16) + (q % 8) * 2;
 #pragma unroll
                 for (int part = 0; part < PARTS; part++) *reinterpret_cast<unsigned short*>(at + part * PART_BYTES) = h[part] >> 16;
             }
+        }
+        if constexpr (!XBF) {
+            if ((left & 0xFFFFu) != 0) leaves[wave] = 1;
         }
     };
     // rows past the end are read as what LDS holds there, or as the last row where R < 16: their sums are not stored
@@ -695,6 +786,12 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, X
             }
         }
     };
+    // what leaves something over is told of in LDS before a slice's barrier, and looked up well before it is asked for
+    unsigned some_leave = 0;  // one wavefront's to a lane
+    auto look = [&] {
+        if constexpr (!XBF) some_leave = leaves[lane % WAVES];
+    };
+    if constexpr (!XBF) leaves[wave] = 0;
     int turn = 0;
     auto work_on = [&](const char* slice, int base) {
         const int stop = min(turns_all, turn + (1 << log_turns));
@@ -720,6 +817,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, X
                 load_scales(base + 2 * SLICE);
                 load_x(base + 2 * SLICE);
             }
+            look();
             if (base >= first) work_on(lds + here, base);
             __syncthreads();
             const int before = here;
@@ -734,6 +832,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, X
                 load_x(base + SLICE);
             }
             if (base >= first) {
+                look();
                 work_on(lds, base);
                 __syncthreads();
             }
@@ -747,12 +846,27 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, X
 
     // lane (ln, lj) holds column ln, rows 4 lj .. 4 lj + 3 of each 16 x 16 tile; the wavefronts of a column add up
     f32x4* sums = reinterpret_cast<f32x4*>(lds);  // [wavefronts][NT][64]
-#pragma unroll
-    for (int i = 0; i < MT; i++) {
-        if (i) __syncthreads();
+    auto put_sums = [&](int i) {
 #pragma unroll
         for (int t = 0; t < NT; t++) sums[(wave * NT + t) * 64 + lane] = acc[i][t];
-        __syncthreads();
+    };
+    put_sums(0);
+    __syncthreads();
+    if constexpr (!XBF) {
+        if (__builtin_expect(__any(some_leave != 0), 0)) {
+            add_left_over<R, MT, NT, GROUP>(lds, acc);
+            __syncthreads();
+            put_sums(0);
+            __syncthreads();
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; i++) {
+        if (i) {
+            __syncthreads();
+            put_sums(i);
+            __syncthreads();
+        }
         for (int e = threadIdx.x; e < columns * NT * 64; e += 64 * WAVES) {
             const int group = e / (NT * 64), rest = e % (NT * 64);
             f32x4 y = sums[group * kw * NT * 64 + rest];
