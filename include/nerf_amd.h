@@ -170,7 +170,8 @@ void nerf_adamw_destroy(NerfAdamw* plan);
  * in m_exp / v_exp).  seed 0 rounds to nearest (ties away from zero); another seed rounds up or down by chance, a
  * pure function of (seed, step, place in the list, element), so that changes smaller than a rounding step are not
  * lost on average: what training wants, as v moves by a thousandth a step.  A sqrt(v) that is not zero stays so; a
- * moment that is not finite is held as zero.  seed is not used with 32-bit states.
+ * moment that is not finite is held as zero, and an m beside a sqrt(v) that is held as zero counts as zero: after a gradient
+ * whose square is too large both start again.  seed is not used with 32-bit states.
  * d_norm: one float on the device (nerf_grad_norm) or NULL; then max_norm is not used.
  * Returns 1 while the stream is being captured: a graph would repeat this step number and learning rate. */
 int nerf_adamw_step(NerfAdamw* plan, int step, float learning_rate, float grad_div, const float* d_norm, float max_norm,

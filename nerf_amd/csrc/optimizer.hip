@@ -236,8 +236,15 @@ __global__ __launch_bounds__(256) void adamw32_kernel(const StepArgs a) {
 //             divides by keeps 5 significant bits)
 // An fp32 number whose exponent field is 0..15 holds such a code in its upper bits, so a value becomes a code by
 // scaling it with 2^(15-E) and rounding off the lower mantissa bits, carry and underflow included.
+// A root's code is zero only where v is, or was not finite; v is zero only where every gradient so far was, or next to it (or
+// beta2 forgets it at once).  An m beside such a code counts as zero, whatever its own code: what the update divides it by
+// is gone (the step after a gradient of 1e21 would divide 1e20 by eps).
 __device__ __forceinline__ float decode(unsigned code, int low, int exponent) {
     return __builtin_amdgcn_ldexpf(__builtin_bit_cast(float, code << low), exponent - 15);
+}
+__device__ __forceinline__ float decode_m(unsigned code, unsigned root_code, int exponent) {
+    const float x = root_code ? decode(code & 127, 20, exponent) : 0.0f;
+    return code & 128 ? -x : x;
 }
 __device__ __forceinline__ unsigned encode(float x, int low, int exponent, unsigned noise) {
     return (__builtin_bit_cast(unsigned, __builtin_amdgcn_ldexpf(x, 15 - exponent)) + noise) >> low;
@@ -282,10 +289,10 @@ __device__ __forceinline__ void adamw8_block(const StepArgs& a, const Piece& p, 
 #pragma unroll
     for (int k = 0; k < 4; k++) {
         const unsigned mb = (m_old >> (8 * k)) & 255, vb = (v_old >> (8 * k)) & 255;
-        const float m0 = decode(mb & 127, 20, m_e);
+        const float m0 = decode_m(mb, vb, m_e);
         const float r0 = decode(vb, 19, v_e);
         const float gi = gradient(a, g[k], p.factor);
-        m[k] = __fadd_rn(__fmul_rn(a.beta1, mb & 128 ? -m0 : m0), __fmul_rn(c1, gi));
+        m[k] = __fadd_rn(__fmul_rn(a.beta1, m0), __fmul_rn(c1, gi));
         r[k] = sqrtf(__fadd_rn(__fmul_rn(a.beta2, __fmul_rn(r0, r0)), __fmul_rn(__fmul_rn(c2, gi), gi)));
         const float up = __fdiv_rn(__fmul_rn(p.alpha, m[k]), __fadd_rn(r[k], a.eps));
         w[k] = __fsub_rn(__fmul_rn(w[k], p.decay), up);
@@ -346,8 +353,7 @@ __global__ __launch_bounds__(256) void read_states_kernel(const Chunk* chunks, u
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             const unsigned mb = (mc >> (8 * k)) & 255, vb = (vc >> (8 * k)) & 255;
-            const float x = decode(mb & 127, 20, m_e);
-            m[k] = mb & 128 ? -x : x;
+            m[k] = decode_m(mb, vb, m_e);
             r[k] = decode(vb, 19, v_e);
         }
         if (m_out) store4_bf16<STREAM>(m_out + c.first + i, m, left);
