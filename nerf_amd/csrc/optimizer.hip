@@ -368,7 +368,15 @@ __global__ __launch_bounds__(256) void read_states_kernel(const Chunk* chunks, u
 // ---- global norm ----------------------------------------------------------------------------------------
 // Squares are added in 64 bits, so neither the range of the squares nor the length of the sum costs anything
 // (the kernel waits for memory).  Each wavefront walks the pieces at a fixed stride, each workgroup leaves one partial sum;
-// the workgroup that finishes last adds the partial sums in their order: the same bits on every call.
+// the workgroup that draws the last ticket adds the partial sums in their order: the same bits on every call.
+//
+// A partial sum is all that passes between workgroups, and it says itself that it is there: its place holds NO_SUM until then,
+// and again as soon as it is taken.  So nothing hangs on the order in which operations on different places are seen, only
+// on one place's own: no fence is needed, which would write the caches back.  The last one's loads nearly always come
+// after all sums; where one does not, it asks again, and the sum it asks for is on its way: its workgroup sent it before it drew
+// its ticket.  (Two calls at once on one plan, which are not allowed, could take each other's sums, so the asking ends.)
+constexpr unsigned long long NO_SUM = ~0ull;  // a NaN that no sum of squares is: its lower bits come from doubles made of floats
+constexpr int MOST_TURNS = 1 << 16;
 __device__ __forceinline__ double block_sum(double x, double* shared) {
 #pragma unroll
     for (int d = 32; d >= 1; d >>= 1) x += __shfl_xor(x, d, 64);
@@ -421,20 +429,18 @@ __global__ __launch_bounds__(64 * NORM_WAVES) void grad_norm_kernel(const Chunk*
     }
     sum = block_sum(sum, shared);
     if (threadIdx.x == 0) {
-        // The partial sum goes out, and comes in below, by atomic operations of the whole GPU, and the ticket is drawn
-        // when the exchange has answered (its answer is part of the limit, as zero): all that has to be seen is
-        // at the point where those meet, and no cache has to be written back.
-        const unsigned long long before = __hip_atomic_exchange(partial + blockIdx.x, __builtin_bit_cast(unsigned long long, sum),
-                                                                __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        unsigned none = (unsigned)before;
-        asm volatile("v_and_b32 %0, 0, %0" : "+v"(none));
-        last = atomicInc(ticket, gridDim.x - 1 + none) == gridDim.x - 1;  // the last one takes it back to 0 for the next call
+        __hip_atomic_store(partial + blockIdx.x, __builtin_bit_cast(unsigned long long, sum), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last = atomicInc(ticket, gridDim.x - 1) == gridDim.x - 1;  // the last one takes it back to 0 for the next call
     }
     __syncthreads();
     if (!last) return;
     sum = 0.0;
-    for (unsigned b = threadIdx.x; b < gridDim.x; b += 64 * NORM_WAVES)
-        sum += __builtin_bit_cast(double, __hip_atomic_load(partial + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    for (unsigned b = threadIdx.x; b < gridDim.x; b += 64 * NORM_WAVES) {
+        unsigned long long bits = NO_SUM;
+        for (int turn = 0; bits == NO_SUM && turn < MOST_TURNS; turn++) bits = __hip_atomic_load(partial + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(partial + b, NO_SUM, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        sum += __builtin_bit_cast(double, bits);
+    }
     sum = block_sum(sum, shared);
     if (threadIdx.x == 0) *norm = (float)(sqrt(sum) / (double)grad_div);
 }
@@ -555,6 +561,7 @@ static int build_plan(const NerfAdamwTensor* tensors, int count, int state_bits,
     }
     constexpr size_t HEAD = NORM_BLOCKS * sizeof(unsigned long long) + 256;
     std::vector<char> image(HEAD + pieces * sizeof(Chunk));
+    std::fill_n(reinterpret_cast<unsigned long long*>(image.data()), NORM_BLOCKS, NO_SUM);
     Chunk* table = reinterpret_cast<Chunk*>(image.data() + HEAD);
     DevicePointers known(plan->device);
     size_t first = 0;
