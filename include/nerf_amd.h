@@ -200,9 +200,9 @@ int nerf_dequantize_w4(const unsigned char* d_codes, const unsigned short* d_sca
 /* Y[M][N] = act(X[M][K] W[N][K]^T) for W in 4 bits: x_type and y_type NERF_TYPE_*, rows ldx >= K and ldy >= N elements
  * apart, epilogue 0: act is nothing, 1: swish.  Products are exact, sums are in fp32 and Y is rounded once.  Made for
  * few rows (one to some dozens); for hundreds, dequantize once and use nerf_gemm_f32 or nerf_gemm_bf16_nt.  Needs
- * d_codes 16-byte aligned.  d_workspace: nerf_gemm_w4_workspace bytes, 16-byte aligned (may be NULL where that is 0);
- * calls that overlap in time need one each, replays of captured ones included.  Y overlaps neither an input nor the
- * workspace. */
+ * d_codes 16-byte aligned.  d_workspace: nerf_gemm_w4_workspace bytes, 16-byte aligned (may be NULL where that is 0); these are
+ * at most 16 MiB and never fewer for a larger M, N or K, so the largest call's serves all; calls that overlap in time need
+ * one each, replays of captured ones included.  Y overlaps neither an input nor the workspace. */
 size_t nerf_gemm_w4_workspace(int M, int N, int K);
 int nerf_gemm_w4(const void* d_X, int x_type, long ldx, const unsigned char* d_codes, const unsigned short* d_scales,
                  int group, void* d_Y, int y_type, long ldy, int M, int N, int K, int epilogue, void* d_workspace,

@@ -1029,7 +1029,6 @@ hipError_t launch_gemv(const W4Args& a) {
     return hipGetLastError();
 }
 
-size_t plan_bytes(const GemmPlan& p, int M, int N) { return p.parts > 1 ? (size_t)p.parts * M * N * sizeof(float) : 0; }
 bool group_ok(int group) { return group == 32 || group == 64 || group == 128; }
 bool type_ok(int t) { return t == NERF_TYPE_F32 || t == NERF_TYPE_BF16; }
 int ceil_div(int a, int b) { return a / b + (a % b != 0); }
@@ -1078,8 +1077,14 @@ int nerf_dequantize_w4(const unsigned char* d_codes, const unsigned short* d_sca
 }
 
 size_t nerf_gemm_w4_workspace(int M, int N, int K) {
-    if (M <= 2 || N <= 0 || K <= 0) return 0;
-    return std::max(plan_bytes(plan_gemm(M, N, K, false), M, N), plan_bytes(plan_gemm(M, N, K, true), M, N));
+    const int chunks = ceil_div(std::max(K, 0), 128);
+    if (M <= 2 || N <= 0 || chunks < 2) return 0;
+    // Fewer rows may be split into more parts, and a workspace for many rows has to serve fewer: so this is not the plan's own
+    // size but a bound that grows with each of the three.  A plan has at most min(64, chunks) parts; where it has several,
+    // its workgroups times its parts are at most CUS, and a workgroup has at most 64 x 256 values.
+    const size_t workgroups = (size_t)CUS * std::min(M, 64) * std::min(N, 256), parts = std::min(64, chunks);
+    const size_t values = (size_t)M * N;  // below 2^61
+    return sizeof(float) * (values > workgroups / parts ? workgroups : values * parts);
 }
 
 int nerf_gemm_w4(const void* d_X, int x_type, long ldx, const unsigned char* d_codes, const unsigned short* d_scales,
@@ -1092,7 +1097,7 @@ int nerf_gemm_w4(const void* d_X, int x_type, long ldx, const unsigned char* d_c
         return NERF_ERR_ARG;
     GemmPlan p = {};
     if (M > 2) p = plan_gemm(M, N, K, x_type == NERF_TYPE_BF16);
-    const size_t need = plan_bytes(p, M, N);
+    const size_t need = nerf_gemm_w4_workspace(M, N, K);
     if (workspace_bytes < need || (need && !d_workspace)) return NERF_ERR_ARG;
     W4Args a = {};
     a.X = d_X; a.codes = d_codes; a.scales = d_scales; a.Y = d_Y;
