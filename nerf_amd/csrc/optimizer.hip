@@ -546,10 +546,15 @@ extern "C" {
 
 size_t nerf_adamw_state_blocks(size_t n) { return n / BLOCK + (n % BLOCK != 0); }
 
-// NERF_OK, or NERF_ERR_ARG while the library's stream is being captured into a graph
+// NERF_OK, or NERF_ERR_ARG while the library's stream is being captured into a graph, or is the default one and another
+// stream that waits for it is captured: the runtime answers that with an error, which is not left for a later call to report
 static int not_capturing() {
     hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(stream(), &capturing) != hipSuccess) return NERF_ERR_HIP;
+    const hipError_t rc = hipStreamIsCapturing(stream(), &capturing);
+    if (rc != hipSuccess) {
+        (void)hipGetLastError();
+        return rc == hipErrorStreamCaptureImplicit ? NERF_ERR_ARG : NERF_ERR_HIP;
+    }
     return capturing == hipStreamCaptureStatusNone ? NERF_OK : NERF_ERR_ARG;
 }
 
@@ -636,8 +641,8 @@ int nerf_adamw_create(const NerfAdamwTensor* tensors, int count, int state_bits,
         rc = NERF_ERR_HIP;
     }
     if (rc != NERF_OK) {
-        (void)hipGetLastError();
         nerf_adamw_destroy(plan);
+        (void)hipGetLastError();
         return rc;
     }
     *out = plan;
@@ -646,7 +651,7 @@ int nerf_adamw_create(const NerfAdamwTensor* tensors, int count, int state_bits,
 
 void nerf_adamw_destroy(NerfAdamw* plan) {
     if (!plan) return;
-    (void)hipFree(plan->memory);
+    if (plan->memory) (void)hipFree(plan->memory);  // of none, too, it would end another stream's capture
     delete plan;
 }
 
