@@ -664,7 +664,7 @@ static bool plan_usable(const NerfAdamw* plan) {
 int nerf_adamw_step(NerfAdamw* plan, int step, float learning_rate, float grad_div, const float* d_norm, float max_norm,
                     unsigned long long seed) {
     if (!plan || !plan->state_bits || step < 1 || !finite_not_negative(learning_rate) || !(grad_div > 0.0f && grad_div < INFINITY) ||
-        (d_norm && !(max_norm > 0.0f && max_norm < INFINITY)) || !plan_usable(plan))
+        (d_norm && (((uintptr_t)d_norm & 3) || !(max_norm > 0.0f && max_norm < INFINITY))) || !plan_usable(plan))
         return NERF_ERR_ARG;
     const int rc = not_capturing();  // a graph would repeat this step number and learning rate for ever
     if (rc != NERF_OK) return rc;

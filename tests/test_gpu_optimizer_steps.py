@@ -66,3 +66,15 @@ def test_a_first_moment_beside_a_root_held_as_zero_counts_as_zero(gpu, seed):
     # check_weights' bound: alpha holds 1 - beta2^3 = 0.003, which loses half a step of beta2^3
     case.w, case.m, case.v = [w], [held], [roots]
     check_weights(case, case.aw.read(), 3, 1e-3, 1.0, 1.0)
+
+
+def test_a_norm_that_is_not_aligned_is_refused(gpu):
+    """a scalar load would read the float before it"""
+    from nerf_amd._lib import lib
+    from nerf_amd.api import DeviceArray
+    case, norm = Case([100], 32, 1), DeviceArray.from_numpy(np.array([1.0, 2.0], np.float32))
+    before = case.aw.read()[0].copy()
+    for shift in (1, 2, 3):
+        assert lib.nerf_adamw_step(case.plan.handle, 1, 1e-3, 1.0, norm.ptr + shift, 1.0, 0) == 1
+    assert np.array_equal(case.aw.read()[0], before)
+    assert lib.nerf_adamw_step(case.plan.handle, 1, 1e-3, 1.0, norm.ptr + 4, 1.0, 0) == 0
