@@ -132,7 +132,7 @@ int nerf_weight_gradient_bf16(const unsigned short* d_err, int rows_out, int ld_
  * matrices of one MLP (train.c:219-220): a list of tensors of any number, sizes and alignment is updated by ONE
  * launch, with the states in 32 or in 8 bits, after an optional clip by the global norm of the gradients. -------- */
 enum { NERF_TYPE_F32 = 0, NERF_TYPE_BF16 = 1 };
-#define NERF_ADAMW_MAX_ELEMENTS ((size_t)1 << 40) /* of one tensor */
+#define NERF_ADAMW_MAX_ELEMENTS ((((size_t)1 << 22) - 1) * 4096) /* of one tensor, and of a list: see nerf_adamw_create */
 typedef struct {
     float* w;              /* weights [n] */
     const void* g;         /* gradients [n], of grad_type */
@@ -152,9 +152,10 @@ size_t nerf_adamw_state_blocks(size_t n);
 /* A plan over `count` tensors on the current device.  state_bits: 32, 8, or 0 for a plan that only takes norms (it
  * reads g, grad_type and n of each tensor).  The list is copied; its pointers (device memory, aligned to their
  * elements) must stay valid while the plan is used, and their contents are the caller's.  Zeroed states are the
- * start.  A list has up to 2^22 - 1 runs of 4096 elements (a tensor's last run may be shorter).  Returns 1 for a bad
- * argument: among them a buffer that a step writes and that overlaps another one of the list, a pointer to pageable host
- * memory or another GPU, a buffer longer than its allocation, and a stream that is being captured. */
+ * start.  A list has up to 2^22 - 1 runs of 4096 elements (a tensor's last run may be shorter: it counts as one).
+ * Returns 1 for a bad argument: among them a buffer that a step writes and that overlaps another one of the list, a
+ * pointer to pageable host memory or another GPU, a buffer longer than its allocation, and a stream that is being
+ * captured. */
 int nerf_adamw_create(const NerfAdamwTensor* tensors, int count, int state_bits, float beta1, float beta2, float eps,
                       NerfAdamw** out);
 /* waits for the device's work and frees the plan's own tables */

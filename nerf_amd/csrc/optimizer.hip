@@ -499,10 +499,13 @@ bool disjoint(std::vector<Range>& r) {
 int check_tensors(const NerfAdamwTensor* tensors, int count, int state_bits) {
     if (!tensors || count < 1 || (state_bits != 0 && state_bits != 8 && state_bits != 32)) return NERF_ERR_ARG;
     std::vector<Range> ranges;
+    size_t chunks = 0;
     for (int k = 0; k < count; k++) {
         const NerfAdamwTensor& t = tensors[k];
         if (t.n == 0) continue;
-        if (t.n > NERF_ADAMW_MAX_ELEMENTS || (t.grad_type != NERF_TYPE_F32 && t.grad_type != NERF_TYPE_BF16)) return NERF_ERR_ARG;
+        if (t.n > NERF_ADAMW_MAX_ELEMENTS) return NERF_ERR_ARG;
+        chunks += t.n / CHUNK + (t.n % CHUNK != 0);
+        if (chunks > NERF_ADAMW_MAX_ELEMENTS / CHUNK || (t.grad_type != NERF_TYPE_F32 && t.grad_type != NERF_TYPE_BF16)) return NERF_ERR_ARG;
         const size_t g_item = t.grad_type == NERF_TYPE_BF16 ? 2 : 4;
         auto add = [&](const void* p, size_t items, size_t item, bool written) {
             const uintptr_t at = (uintptr_t)p;
@@ -559,11 +562,9 @@ static int not_capturing() {
 }
 
 static int build_plan(const NerfAdamwTensor* tensors, int count, int state_bits, NerfAdamw* plan) {
+    static_assert(NERF_ADAMW_MAX_ELEMENTS % CHUNK == 0 && NERF_ADAMW_MAX_ELEMENTS / PIECE * 256 < 1ull << 32, "a launch has fewer than 2^32 threads");
     size_t pieces = 0;
-    for (int k = 0; k < count; k++) {
-        pieces += tensors[k].n / CHUNK + (tensors[k].n % CHUNK != 0);
-        if (pieces > 0xffffffu / PIECES) return NERF_ERR_ARG;  // a launch has fewer than 2^32 threads
-    }
+    for (int k = 0; k < count; k++) pieces += tensors[k].n / CHUNK + (tensors[k].n % CHUNK != 0);
     constexpr size_t HEAD = NORM_BLOCKS * sizeof(unsigned long long) + 256;
     std::vector<char> image(HEAD + pieces * sizeof(Chunk));
     std::fill_n(reinterpret_cast<unsigned long long*>(image.data()), NORM_BLOCKS, NO_SUM);
