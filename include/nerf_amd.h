@@ -170,7 +170,9 @@ void nerf_adamw_destroy(NerfAdamw* plan);
  * 4 exponent bits and 3 mantissa bits, sqrt(v) to 4 and 4, below a power of two per 256 elements (its biased exponent
  * in m_exp / v_exp).  seed 0 rounds to nearest (ties away from zero); another seed rounds up or down by chance, a
  * pure function of (seed, step, place in the list, element), so that changes smaller than a rounding step are not
- * lost on average: what training wants, as v moves by a thousandth a step.  A sqrt(v) that is not zero stays so; a
+ * lost on average: what training wants, as v moves by a thousandth a step.  (Steady gradients: to nearest, sqrt(v) falls to
+ * 0.68 of its value in 300 steps and to 0.50 in 4000, so that weights move twice as far; by chance it stays right on
+ * average, nine elements of ten within 20 %.)  A sqrt(v) that is not zero stays so; a
  * moment that is not finite is held as zero, and an m beside a sqrt(v) that is held as zero counts as zero: after a gradient
  * whose square is too large both start again.  seed is not used with 32-bit states.
  * d_norm: one float on the device (nerf_grad_norm) or NULL; then max_norm is not used.

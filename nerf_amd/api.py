@@ -5,6 +5,7 @@ Dataset, MLP, generate_random_batch, forward_pass_mlp, ...  Everything numerical
 HIP library; this module only moves numpy arrays in and out and keeps C structs alive.
 """
 import ctypes as C
+import warnings
 
 import numpy as np
 
@@ -333,6 +334,7 @@ class AdamW:
 
     def __init__(self, tensors, state_bits=32, beta1=0.9, beta2=0.999, eps=1e-8):
         self.handle = None
+        self._state_bits = state_bits
         self._keep = list(tensors)
         table = (_lib.NerfAdamwTensor * max(1, len(self._keep)))()
         for t, s in zip(self._keep, table):
@@ -358,7 +360,15 @@ class AdamW:
         except Exception:
             pass
 
-    def step(self, step, lr, grad_div=1.0, norm=None, max_norm=0.0, seed=0):
+    def step(self, step, lr, grad_div=1.0, norm=None, max_norm=0.0, seed=None):
+        """seed: for 8-bit states, any number but 0 rounds them by chance, which training needs; 0 rounds them to nearest,
+        which loses the small changes of v (sqrt(v) falls to half of its value over some thousand steps).  A step with 8-bit
+        states and no seed rounds to nearest and warns."""
+        if seed is None:
+            if self._state_bits == 8:
+                warnings.warn("AdamW.step without a seed rounds 8-bit states to nearest: v loses its small changes, and updates grow "
+                              "up to twofold over some thousand steps; pass a seed that is not 0", stacklevel=2)
+            seed = 0
         _check(lib.nerf_adamw_step(self.handle, step, lr, grad_div, _ptr(norm), max_norm, seed), "nerf_adamw_step")
 
     def grad_norm(self, norm, grad_div=1.0):

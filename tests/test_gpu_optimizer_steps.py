@@ -68,6 +68,52 @@ def test_a_first_moment_beside_a_root_held_as_zero_counts_as_zero(gpu, seed):
     check_weights(case, case.aw.read(), 3, 1e-3, 1.0, 1.0)
 
 
+@pytest.mark.parametrize("bf16", [False, True])
+def test_states_in_8_bits_follow_64_bit_ones_where_a_seed_rounds_by_chance(gpu, bf16):
+    """300 steps of steady gradients.  Rounding by chance is right on average; what a step adds to the variance of sqrt(v) is at
+    most a step of the code (1/16 of the value at most) times the mean change, 0.97 / 2 thousandths of the value and up to
+    1 / 2t in the first t steps, and v forgets a thousandth a step: at most 6 % of v, 3 % of its root, and the mean of 4096
+    roots that scatter by 12 % is 0.2 % off.  To nearest, where no change is as large as half a step, the mean falls below 0.8."""
+    torch = pytest.importorskip("torch")
+    from nerf_amd._lib import lib
+    from nerf_amd.api import AdamW
+    n, lr = 4096, 1e-3
+    blocks = lib.nerf_adamw_state_blocks(n)
+    new = lambda count, t: torch.zeros(count, dtype=t, device="cuda")  # noqa: E731
+    ratio = {}
+    for seed in (0, 17):
+        gen = torch.Generator(device="cuda").manual_seed(9)
+        w, g = new(n, torch.float32), new(n, torch.bfloat16 if bf16 else torch.float32)
+        m, v, me, ve = new(n, torch.uint8), new(n, torch.uint8), new(blocks, torch.uint8), new(blocks, torch.uint8)
+        right, roots = new(n, torch.float64), new(n, torch.bfloat16)
+        torch.cuda.synchronize()
+        plan = AdamW([dict(w=w.data_ptr(), g=g.data_ptr(), m=m.data_ptr(), v=v.data_ptr(), m_exp=me.data_ptr(), v_exp=ve.data_ptr(), n=n,
+                           g_bf16=bf16)], state_bits=8)
+        b2 = float(np.float32(0.999))
+        for step in range(1, 301):
+            g.copy_(torch.randn(n, device="cuda", generator=gen) * 1e-3)
+            plan.step(step, lr, seed=seed)
+            right.mul_(b2).add_(g.double().square(), alpha=1 - b2)
+        plan.read_states(None, roots.data_ptr())
+        torch.cuda.synchronize()
+        ratio[seed] = (roots.double() / right.sqrt()).mean().item()
+        plan.destroy()
+    assert abs(ratio[17] - 1) <= 0.032, ratio
+    assert ratio[0] < 0.8, ratio  # what the documentation warns of
+
+
+def test_a_step_without_a_seed_warns(gpu):
+    import warnings
+    small, large = Case([300], 8, 5), Case([300], 32, 5)
+    with pytest.warns(UserWarning, match="seed"):
+        small.plan.step(1, 1e-3)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        small.plan.step(2, 1e-3, seed=0)
+        small.plan.step(3, 1e-3, seed=4)
+        large.plan.step(1, 1e-3)
+
+
 def test_a_norm_that_is_not_aligned_is_refused(gpu):
     """a scalar load would read the float before it"""
     from nerf_amd._lib import lib
