@@ -155,7 +155,8 @@ size_t nerf_adamw_state_blocks(size_t n);
  * start.  A list has up to 2^22 - 1 runs of 4096 elements (a tensor's last run may be shorter: it counts as one).
  * Returns 1 for a bad argument: among them a buffer that a step writes and that overlaps another one of the list, a
  * pointer to pageable host memory or another GPU, a buffer longer than its allocation, and a stream that is being
- * captured. */
+ * captured.  A plan costs checks of every buffer, a table in device memory and a wait: 18 us for four tensors, 0.13 ms for
+ * 200, 0.5 ms for 134 million elements.  It is made for addresses that stay; a list whose addresses move needs another. */
 int nerf_adamw_create(const NerfAdamwTensor* tensors, int count, int state_bits, float beta1, float beta2, float eps,
                       NerfAdamw** out);
 /* waits for the device's work and frees the plan's own tables */
@@ -172,10 +173,10 @@ void nerf_adamw_destroy(NerfAdamw* plan);
  * pure function of (seed, step, place in the list, element), so that changes smaller than a rounding step are not
  * lost on average: what training wants, as v moves by a thousandth a step.  (Steady gradients: to nearest, sqrt(v) falls to
  * 0.68 of its value in 300 steps and to 0.50 in 4000, so that weights move twice as far; by chance it stays right on
- * average, nine elements of ten within 20 %.)  A sqrt(v) that is not zero stays so; a
- * moment that is not finite is held as zero, and an m beside a sqrt(v) that is held as zero counts as zero: after a gradient
- * whose square is too large both start again.  seed is not used with 32-bit states.
- * d_norm: one float on the device (nerf_grad_norm) or NULL; then max_norm is not used.
+ * average, nine elements of ten within 20 %.)  A new sqrt(v) that is not zero in fp32 (v of 1e-45 and more) is not rounded
+ * to zero.  A moment that is not finite is held as zero, and an m beside a sqrt(v) that is held as zero counts as zero: after
+ * a gradient whose square is too large both start again.  seed is not used with 32-bit states.
+ * d_norm: one float on the device (nerf_grad_norm), aligned, or NULL; then max_norm is not used.
  * Returns 1 while the stream is being captured: a graph would repeat this step number and learning rate. */
 int nerf_adamw_step(NerfAdamw* plan, int step, float learning_rate, float grad_div, const float* d_norm, float max_norm,
                     unsigned long long seed);
@@ -197,11 +198,13 @@ size_t nerf_w4_row_bytes(int cols); /* 16 bytes per 32 columns, rounded up */
  * apart; codes behind the last column are zero.  d_codes must be 16-byte aligned. */
 int nerf_quantize_w4(const float* d_src, long ld_src, int rows, int cols, int group, unsigned char* d_codes,
                      unsigned short* d_scales);
-/* the weights that the codes stand for, in fp32 (exact) */
+/* the weights that the codes stand for, in fp32 (exact; weights above 3.38e38 may come back as infinities, since their scale
+ * times 6 is no fp32 number) */
 int nerf_dequantize_w4(const unsigned char* d_codes, const unsigned short* d_scales, int rows, int cols, int group,
                        float* d_dst, long ld_dst);
 /* Y[M][N] = act(X[M][K] W[N][K]^T) for W in 4 bits: x_type and y_type NERF_TYPE_*, rows ldx >= K and ldy >= N elements
- * apart, epilogue 0: act is nothing, 1: swish.  Products are exact, sums are in fp32 and Y is rounded once.  Made for
+ * apart, epilogue 0: act is nothing, 1: swish.  Products are exact, sums are in fp32 and Y is rounded once; a group's
+ * sum is taken before its scale, so X has to stay below 2^118 in magnitude (3e35) not to overflow there.  Made for
  * few rows (one to some dozens); for hundreds, dequantize once and use nerf_gemm_f32 or nerf_gemm_bf16_nt.  Needs
  * d_codes 16-byte aligned.  d_workspace: nerf_gemm_w4_workspace bytes, 16-byte aligned (may be NULL where that is 0); these are
  * at most 16 MiB and never fewer for a larger M, N or K, so the largest call's serves all; calls that overlap in time need

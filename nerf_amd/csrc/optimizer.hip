@@ -79,7 +79,7 @@ __device__ __forceinline__ unsigned short f32_to_bf16(float x) {
     return __builtin_bit_cast(unsigned short, (__bf16)x);  // to nearest, ties to even
 }
 
-// a 32-bit mixing function: xor-shifts and two odd multipliers
+// a 32-bit mixing function, xor-shifts and two odd multipliers: the published integer hash lowbias32
 __host__ __device__ __forceinline__ unsigned mix32(unsigned x) {
     x ^= x >> 16;
     x *= 0x7FEB352Du;
@@ -683,7 +683,7 @@ int nerf_adamw_step(NerfAdamw* plan, int step, float learning_rate, float grad_d
     a.eps = plan->eps;
     a.norm = d_norm;
     a.max_norm = max_norm;
-    // one 32-bit key per (seed, step): a 64-bit mixing function, its halves folded
+    // one 32-bit key per (seed, step): a 64-bit mixing function (splitmix64), its halves folded
     unsigned long long z = seed + (unsigned long long)step * 0x9E3779B97F4A7C15ull;
     z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
     z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;

@@ -124,3 +124,27 @@ def test_a_norm_that_is_not_aligned_is_refused(gpu):
         assert lib.nerf_adamw_step(case.plan.handle, 1, 1e-3, 1.0, norm.ptr + shift, 1.0, 0) == 1
     assert np.array_equal(case.aw.read()[0], before)
     assert lib.nerf_adamw_step(case.plan.handle, 1, 1e-3, 1.0, norm.ptr + 4, 1.0, 0) == 0
+
+
+def test_training_goes_on_bit_for_bit_from_states_that_were_copied_out(gpu):
+    """what a checkpoint of an outside plan has to hold: weights, codes, exponents, the step number and the seed"""
+    sizes = [700, 5000]
+    rng = np.random.default_rng(3)
+    gradients = [[rng.normal(0, 1e-2, n).astype(np.float32) for n in sizes] for _ in range(6)]
+
+    def steps(case, first, last):
+        for step in range(first, last):
+            flat = case.ag.dev.numpy()
+            flat[case.ag.start:case.ag.start + sum(sizes)] = np.concatenate(gradients[step - 1])
+            case.ag.dev.upload(flat)
+            case.plan.step(step, 1e-3, seed=5)
+
+    one, two = Case(sizes, 8, 31), Case(sizes, 8, 32)  # two starts with other contents
+    steps(one, 1, 4)
+    arenas = lambda case: (case.aw, case.am, case.av, case.ame, case.ave)  # noqa: E731
+    for a, b in zip(arenas(one), arenas(two)):
+        b.dev.upload(a.dev.numpy())
+    steps(one, 4, 7)
+    steps(two, 4, 7)
+    for a, b in zip(arenas(one), arenas(two)):
+        assert np.array_equal(a.dev.numpy(), b.dev.numpy())

@@ -1,4 +1,4 @@
-"""GPU: products of rows whose values are all small.  No part of an input is lost whatever its size, so the bound is the one
+"""GPU: products of rows whose values are all small, and of the largest that are allowed.  No part of an input is lost whatever its size, so the bound is the one
 of ordinary rows, relative to the sum of magnitudes."""
 import numpy as np
 import pytest
@@ -23,12 +23,12 @@ def large_weights(n, k, seed):
     return (rng.normal(size=(n, k)) * 1e30).astype(np.float32)
 
 
-@pytest.mark.parametrize("bf16", [False, True])
+SIZES = [1e-33, 1e-34, 1e-35, 1e-36, 1e-37, 1e-38, 1e-39, 1e-40, 1e-42, 1e-44]
+
+
 @pytest.mark.parametrize("m", [1, 2, 3, 6, 20, 40])
-@pytest.mark.parametrize("size", [1e-33, 1e-34, 1e-35, 1e-36, 1e-37, 1e-38, 1e-39, 1e-40, 1e-42, 1e-44])
-def test_rows_of_small_values(gpu, size, m, bf16):
-    if bf16 and size < 2.0 ** -133:
-        pytest.skip("below the smallest bf16 number")
+@pytest.mark.parametrize("size,bf16", [(s, False) for s in SIZES] + [(s, True) for s in SIZES if s > 2.0 ** -133])
+def test_rows_of_small_values(gpu, size, bf16, m):
     n, k = 37, 200
     codes, scales = ref.quantize_w4(large_weights(n, k, 3), 32)
     w = ref.dequantize_w4(codes, scales, k, 32)
@@ -102,3 +102,33 @@ def test_small_values_with_scales_that_are_small_too(gpu, m):
     got = run(x, codes, scales, group, n, k, False, False, 0)
     assert (got[:, ::2] == 0).all()
     check(got[:, 1::2], x.astype(np.float64), ref.dequantize_w4(codes, scales, k, group)[1::2], False, 0)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("m", [1, 2, 3, 20, 64])
+def test_rows_of_the_largest_values(gpu, m, group, bf16):
+    """all of one sign and just below 2^118, against the largest code: the sum of a group of 128 is below 2^128"""
+    n, k = 20, 300
+    w = np.random.default_rng(4).uniform(5.5e-6, 6e-6, (n, k)).astype(np.float32)
+    codes, scales = ref.quantize_w4(w, group)
+    w = ref.dequantize_w4(codes, scales, k, group)
+    x = np.random.default_rng(m).uniform(0.9, 0.99, (m, k)).astype(np.float32) * np.float32(2.0 ** 118)
+    held = ref.bf16(x) if bf16 else x
+    x = ref.from_bf16(held) if bf16 else x
+    check(run(held, codes, scales, group, n, k, bf16, False, 0), x.astype(np.float64), w, False, 0)
+
+
+def test_dequantize_of_the_largest_weights(gpu):
+    """6 times a bf16 scale is an fp32 number up to 255 / 256 of 2^128: 3.38e38 comes back, fp32's largest as an infinity"""
+    from nerf_amd._lib import lib
+    from nerf_amd.api import DeviceArray
+    w = np.zeros((2, 32), np.float32)
+    w[0, :3] = [3.38e38, -3.38e38, 1e38]
+    w[1, :2] = np.finfo(np.float32).max
+    d, codes, scales, back = DeviceArray.from_numpy(w), DeviceArray((2, 16), np.uint8), DeviceArray((2, 1), np.uint16), DeviceArray((2, 32))
+    assert lib.nerf_quantize_w4(d.ptr, 32, 2, 32, 32, codes.ptr, scales.ptr) == 0
+    assert lib.nerf_dequantize_w4(codes.ptr, scales.ptr, 2, 32, 32, back.ptr, 32) == 0
+    got, want = back.numpy(), ref.dequantize_w4(codes.numpy(), scales.numpy(), 32, 32)
+    assert np.array_equal(got[0].astype(np.float64), want[0]) and np.isfinite(got[0]).all()
+    assert np.isposinf(got[1, :2]).all() and (want[1, :2] > np.finfo(np.float32).max).all()
