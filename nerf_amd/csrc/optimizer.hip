@@ -7,8 +7,8 @@
 //
 // Everything here waits for memory.  A workgroup takes 1024 elements, four to a thread: all it reads is asked for
 // before the first use, and there are always others to take over while it waits (134 million elements, bf16 gradients
-// and copy, 28 bytes an element: 623 us = 6.0 TB/s; with 2048, 4096 and 8192 elements to a workgroup 658, 671 and
-// 684 us; a loop over the pieces does not overlap them as well as the scheduler does).
+// and copy, 28 bytes an element: 593 us = 6.3 TB/s, 580 to 645 over cards; on one card 623 us, and with 2048, 4096 and 8192
+// elements to a workgroup 658, 671 and 684; a loop over the pieces does not overlap them as well as the scheduler does).
 #include "common.hpp"
 #include "../../include/nerf_amd.h"
 
@@ -238,7 +238,8 @@ __global__ __launch_bounds__(256) void adamw32_kernel(const StepArgs a) {
 // scaling it with 2^(15-E) and rounding off the lower mantissa bits, carry and underflow included.
 // A root's code is zero only where v is, or was not finite; v is zero only where every gradient so far was, or next to it (or
 // beta2 forgets it at once).  An m beside such a code counts as zero, whatever its own code: what the update divides it by
-// is gone (the step after a gradient of 1e21 would divide 1e20 by eps).
+// is gone (the step after a gradient of 1e21 would divide 1e20 by eps).  This costs the step of 134 million elements 1.4 %
+// (371 and 376 us; a test of four codes at once before the selections costs as much, and half of the read of states).
 __device__ __forceinline__ float decode(unsigned code, int low, int exponent) {
     return __builtin_amdgcn_ldexpf(__builtin_bit_cast(float, code << low), exponent - 15);
 }
@@ -531,7 +532,7 @@ using namespace nerf;
 
 // Bytes of a step beyond which it streams past the caches (256 MB on the memory side).  Three lists in turn, each with
 // and without: 4 million elements in 32 bits (112 MB) 19.8 and 18.1 us, 8 million (224 MB) 37.7 and 43.3 us, 134 million with
-// bf16 gradients and copy (3.8 GB) 623 and 739 us.
+// bf16 gradients and copy (3.8 GB) 623 and 739 us (one card).
 constexpr double STREAM_BYTES = 160e6;
 
 struct NerfAdamw {
@@ -723,7 +724,8 @@ int nerf_grad_norm(NerfAdamw* plan, float grad_div, float* d_norm) {
     // A piece to a wavefront up to one workgroup per CU, two workgroups for long lists: every workgroup adds 10 ns for its
     // ticket, every further round of pieces the time of a read.  134 million bf16 elements take 94.9, 55.5, 46.9 and 49.7 us
     // with at most 128, 256, 512 and 1024 workgroups (5.7 TB/s), 16 million in fp32 13.2, 13.8, 15.4 and 19.3 us, 603 136
-    // (37 workgroups) 4.9 us; workgroups of four wavefronts took 60 and 16.7 us at their best.
+    // (37 workgroups) 4.9 us; workgroups of four wavefronts took 60 and 16.7 us at their best.  (Then a workgroup still waited for
+    // its sum to arrive before it drew its ticket; without that 46.8, 13.4 and 4.5 us.)
     const unsigned pieces = plan->chunks * PIECES, most = pieces < 65536 ? 256 : NORM_BLOCKS;
     const unsigned blocks = std::max(1u, std::min((pieces + NORM_WAVES - 1) / NORM_WAVES, most));
     ProfScope prof(K_GRAD_NORM, plan->grad_bytes);

@@ -365,9 +365,9 @@ __global__ __launch_bounds__(64 * WAVES) void gemv_w4_kernel(const W4Args a, con
 // (16 x 16 x 32), so that a step's 32 columns lie in one group and the sum over a group takes one scale.  Columns of
 // workgroups start at different chunks of a slice: rows of W are often a power of two apart, and workgroups that walk
 // them in step would all ask the same few memory channels.
-//   Times (groups of 64): 16 x 16384 x 8192 23.6 us = 3.0 TB/s of W; left out by turns, X costs 7 us of it, matrix instructions
-// and conversions 4.5, and W, two launches and the join the rest.  24 x 4100 x 4090 13.8 us: X 4, the second
-// launch and the join 4.5, the rest a chain that is too short to overlap.  64 x 16384 x 8192 55.5 us, in bf16 33 = 520 TFLOP/s.
+//   Times (groups of 64): 16 x 16384 x 8192 24.4 us = 2.9 TB/s of W; left out by turns, X costs 7 us of it, matrix instructions
+// and conversions 4.5, and W, two launches and the join the rest.  24 x 4100 x 4090 13.9 us: X 4, the second
+// launch and the join 4.5, the rest a chain that is too short to overlap.  64 x 16384 x 8192 58 us, in bf16 33 = 520 TFLOP/s.
 // Scales that each wavefront loads for itself, chunk by chunk (16 lines for 64 bytes of each row), had cost 5 us of
 // 8 x 16384 x 8192 in bf16 (17.6 us); sixteen wavefronts to a workgroup, or a whole slice of W ahead, gained nothing.
 // eight codes as eight bf16
@@ -545,7 +545,8 @@ struct GemmArguments {  // as they lie in memory
 // The products with what the parts of X leave over, its 16 bits as two parts, slice by slice and nothing ahead: rare.  It
 // reads the arguments again, so that its needs take no registers from what runs before it: inside the main loop, as its second
 // time round, it cost every call 1 us.  Seeing that there is something costs 0.1 to 0.2 us (16 x 512 x 512 4.15 us without and
-// 4.28 with, 24 x 4100 x 4090 13.8 and 14.1, 64 x 16384 x 8192 57.8 and 59.3).
+// 4.28 with, 24 x 4100 x 4090 13.8 and 14.1, 64 x 16384 x 8192 57.8 and 59.3); where a workgroup's X has such numbers the call
+// takes 2.4 to 4 times as long (10.3, 33 and 230).
 template <int R, int MT, int NT, int GROUP>
 __device__ __forceinline__ void add_left_over(char* lds, f32x4 (&acc)[MT][NT]) {
     constexpr int SLICE = slice_chunks(R, MT, false), TILE_BYTES = R * 64, PART_BYTES = MT * TILE_BYTES, STEP_BYTES = 2 * PART_BYTES + 16;
@@ -930,12 +931,15 @@ struct GemmPlan {
 // (multiplied), for a tile of X read from LDS for 16 NT columns, for a slice, for the second kernel that joins parts, for a part,
 // and for a value of one (written and read).  The numbers are fitted to 3600 measured launches of 41 shapes (3 to 200
 // rows, 200 to 32768 columns, K from 500 to 16384) so that the shapes they find are the fastest ones measured: they
-// are within 5 % of those for 36 of them and within 10 % for all.  What decides, with both sides measured (X in fp32):
-//   rows to a workgroup: 64 x 16384 x 8192 61 us with 64 and 72 with 16, but 64 x 512 x 512 4.3 with 16 and 7.6 with 32
-//   columns of a wavefront, 16 or 32: 16 x 16384 x 8192 31.1 and 25.8 us, but 64 x 512 x 512 4.3 and 4.9
-//   wavefronts along the contraction: 3 x 4096 x 4096 6.2, 7.5, 10.5 and 16.6 us with 8, 4, 2 and 1; 16 x 16384 x 8192 25.8 with 1
-// and 30.6 with 2
-//   parts: 24 x 4100 x 4090 38.6, 24.3, 14.4 and 18.6 us with 1, 2, 6 and 12
+// were within 5 % of those for 36 of them and within 10 % for all.  (That was before the present order of X in LDS, and before
+// what is left over of X was looked for.)  What decides, with both sides measured on the code as it is (X in fp32); the shapes
+// found are the fastest of these or within 1 %:
+//   rows to a workgroup: 64 x 16384 x 8192 58.2 us with 64, 58.1 with 32 and 64.6 with 16, but 64 x 512 x 512 4.3 with 16 and 7.4
+// with 32
+//   columns of a wavefront, 16 or 32: 16 x 16384 x 8192 28.0 and 25.0 us, but 64 x 512 x 512 4.3 and 5.2
+//   wavefronts along the contraction: 3 x 4096 x 4096 6.3, 7.7, 10.7 and 16.7 us with 8, 4, 2 and 1; 16 x 16384 x 8192 25.0 with 1
+// and 27.6 with 2
+//   parts: 24 x 4100 x 4090 37.2, 23.6, 14.0 and 18.2 us with 1, 2, 6 and 12
 GemmPlan plan_gemm(int M, int N, int K, bool x_bf16) {
     GemmPlan best = {};
     const int chunks = K / 128 + (K % 128 != 0), r = M <= 4 ? 4 : 16;
